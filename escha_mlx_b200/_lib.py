@@ -68,6 +68,13 @@ SIGNATURES = {
     "escha_debug_gemm_tc_stall": (None, [_i, ctypes.c_uint]),
     "escha_moe_route": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp,
                             _vp, _i, _vp, _sz, _vp]),
+    "escha_page_plan": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
+                             _vp, _vp]),
+    "escha_paged_append": (_i, [_vp, ctypes.c_long, ctypes.c_long, _vp, ctypes.c_long, ctypes.c_long, _i,
+                                _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp]),
+    "escha_paged_attend_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "escha_paged_attend": (_i, [_vp, ctypes.c_long, ctypes.c_long, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp,
+                                _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _vp]),
     "escha_moe_shared_finish": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

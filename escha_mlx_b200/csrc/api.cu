@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../../include/escha_b200.h"
+#include "decode_ops.h"
 #include "kernels.h"
 
 namespace {
@@ -905,6 +906,186 @@ int escha_coded_gemm_tc_status(void) {
     int st = 0;
     if (escha::gemm_tc_status(&st) != cudaSuccess) return -1;
     return st;
+}
+
+// ---- decode step: page plan, paged cache, attention, sampling
+
+namespace {
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+#define REQUIRE_WORDS(p)                                                               \
+    do {                                                                               \
+        if ((p) == nullptr) return fail(ESCHA_EINVAL, "%s: %s is NULL", __func__, #p); \
+        if (!aligned4(p)) return fail(ESCHA_EINVAL, "%s: %s is not 4-byte aligned", __func__, #p); \
+    } while (0)
+
+// log2 of a page size, or -1
+int log_page_of(int page_size) {
+    for (int l = 4; l <= 8; ++l)
+        if (page_size == 1 << l) return l;
+    return -1;
+}
+
+int device_sms() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return sms;
+}
+
+int check_cache(const char* fn, int H, int D, int page_size, int n_pages) {
+    if (D != 64 && D != 128 && D != 256)
+        return fail(ESCHA_EINVAL, "%s: head size %d; the paged cache takes 64, 128 or 256", fn, D);
+    if (H < 1 || H > 1024) return fail(ESCHA_EINVAL, "%s: H=%d outside [1, 1024]", fn, H);
+    if (log_page_of(page_size) < 0)
+        return fail(ESCHA_EINVAL, "%s: page_size=%d is not a power of two in [16, 256]", fn, page_size);
+    if (n_pages < 1 || static_cast<long long>(n_pages) * page_size > 0x7fffffffll)
+        return fail(ESCHA_EINVAL, "%s: n_pages=%d outside [1, 2^31 / page_size)", fn, n_pages);
+    return ESCHA_OK;
+}
+
+int check_types(const char* fn, int type, int cache_type, const float* k_scale, const float* v_scale) {
+    if (type != ESCHA_F16 && type != ESCHA_BF16)
+        return fail(ESCHA_EINVAL, "%s: element type %d is neither binary16 nor bfloat16", fn, type);
+    if (cache_type != type && cache_type != ESCHA_I8)
+        return fail(ESCHA_EINVAL, "%s: a cache of type %d does not go with elements of type %d", fn,
+                    cache_type, type);
+    if (cache_type == ESCHA_I8 && (k_scale == nullptr || v_scale == nullptr))
+        return fail(ESCHA_EINVAL, "%s: an 8-bit cache needs k_scale and v_scale", fn);
+    if (!aligned4(k_scale) || !aligned4(v_scale))
+        return fail(ESCHA_EINVAL, "%s: scales are not 4-byte aligned", fn);
+    return ESCHA_OK;
+}
+
+constexpr long long kMostTokens = 1ll << 30;   // of a request's table
+
+}  // namespace
+
+int escha_page_plan(int32_t* table, const int32_t* lengths, const int32_t* added,
+                    const int32_t* free_pages, int F, const int32_t* head, int B, int W,
+                    int page_size, int n_pages, int rows, int32_t* slots, int32_t* positions,
+                    int32_t* starts, int32_t* ends, int32_t* head_out, int32_t* refused,
+                    void* stream) {
+    REQUIRE(B >= 1 && B <= escha::kPlanMaxBatch, "%s: B=%d outside [1, %d]", __func__, B,
+            escha::kPlanMaxBatch);
+    const int lp = log_page_of(page_size);
+    REQUIRE(lp >= 0, "%s: page_size=%d is not a power of two in [16, 256]", __func__, page_size);
+    REQUIRE(W >= 1 && (static_cast<long long>(W) << lp) <= kMostTokens,
+            "%s: W=%d outside [1, 2^30 / page_size]", __func__, W);
+    REQUIRE(n_pages >= 1 && (static_cast<long long>(n_pages) << lp) <= 0x7fffffffll,
+            "%s: n_pages=%d outside [1, 2^31 / page_size)", __func__, n_pages);
+    REQUIRE(F >= 0, "%s: F=%d is negative", __func__, F);
+    REQUIRE(rows >= 0 && rows <= 1 << 30, "%s: rows=%d outside [0, 2^30]", __func__, rows);
+    REQUIRE_WORDS(table);
+    REQUIRE_WORDS(lengths);
+    REQUIRE_WORDS(added);
+    if (F > 0) REQUIRE_WORDS(free_pages);
+    REQUIRE_WORDS(head);
+    if (rows > 0) {
+        REQUIRE_WORDS(slots);
+        REQUIRE_WORDS(positions);
+    }
+    REQUIRE_WORDS(starts);
+    REQUIRE_WORDS(ends);
+    REQUIRE_WORDS(head_out);
+    REQUIRE_WORDS(refused);
+    escha::PlanParams p{};
+    p.table = table; p.lengths = lengths; p.added = added; p.free_pages = free_pages;
+    p.head = head; p.slots = slots; p.positions = positions; p.starts = starts; p.ends = ends;
+    p.head_out = head_out; p.refused = refused;
+    p.B = B; p.W = W; p.F = F; p.rows = rows; p.log_page = lp; p.n_pages = n_pages;
+    return cuda_result(escha::launch_page_plan(p, as_stream(stream)), "escha_page_plan");
+}
+
+int escha_paged_append(const void* k, long k_row, long k_head, const void* v, long v_row,
+                       long v_head, int in_type, const int32_t* slots, int T, int H, int D,
+                       int page_size, int n_pages, void* k_cache, void* v_cache, int cache_type,
+                       float* k_scale, float* v_scale, void* stream) {
+    if (int rc = check_cache(__func__, H, D, page_size, n_pages)) return rc;
+    if (int rc = check_types(__func__, in_type, cache_type, k_scale, v_scale)) return rc;
+    REQUIRE(T >= 1, "%s: T=%d; at least one row", __func__, T);
+    REQUIRE((k_row | k_head | v_row | v_head) % 8 == 0 && k_row >= 0 && k_head >= 0 && v_row >= 0 &&
+                v_head >= 0,
+            "%s: strides must be multiples of 8 elements", __func__);
+    REQUIRE_PTR(k);
+    REQUIRE_PTR(v);
+    REQUIRE_WORDS(slots);
+    REQUIRE_PTR(k_cache);
+    REQUIRE_PTR(v_cache);
+    escha::AppendParams p{};
+    p.k = k; p.v = v; p.k_row = k_row; p.k_head = k_head; p.v_row = v_row; p.v_head = v_head;
+    p.slots = slots; p.k_cache = k_cache; p.v_cache = v_cache; p.k_scale = k_scale;
+    p.v_scale = v_scale;
+    p.T = T; p.H = H; p.D = D; p.log_page = log_page_of(page_size); p.n_pages = n_pages;
+    return cuda_result(escha::launch_paged_append(p, in_type, cache_type, as_stream(stream)),
+                       "escha_paged_append");
+}
+
+size_t escha_paged_attend_workspace_bytes(int B, int H, int group, int D, int W, int page_size) {
+    const int lp = log_page_of(page_size);
+    if (B < 1 || H < 1 || group < 1 || D < 1 || W < 1 || lp < 0) return 0;
+    const escha::AttendShape s = escha::attend_shape(
+        B < escha::kAttendMaxBatch ? B : escha::kAttendMaxBatch, H, group, D, W, lp, device_sms());
+    return s.meta_bytes + s.ml_bytes + s.part_bytes;
+}
+
+int escha_paged_attend(const void* q, long q_row, long q_head, int q_type, const void* k_cache,
+                       const void* v_cache, int cache_type, const float* k_scale,
+                       const float* v_scale, const int32_t* table, const int32_t* lengths, int B,
+                       int H, int group, int D, int W, int page_size, int n_pages, float scale,
+                       void* workspace, size_t workspace_bytes, void* out, void* stream) {
+    if (int rc = check_cache(__func__, H, D, page_size, n_pages)) return rc;
+    if (int rc = check_types(__func__, q_type, cache_type, k_scale, v_scale)) return rc;
+    REQUIRE(B >= 1 && B <= 1 << 20, "%s: B=%d outside [1, 2^20]", __func__, B);
+    REQUIRE(group >= 1 && group <= 1024, "%s: group=%d outside [1, 1024]", __func__, group);
+    const int lp = log_page_of(page_size);
+    REQUIRE(W >= 1 && (static_cast<long long>(W) << lp) <= kMostTokens,
+            "%s: W=%d outside [1, 2^30 / page_size]", __func__, W);
+    REQUIRE((q_row | q_head) % 8 == 0 && q_row >= 0 && q_head >= 0,
+            "%s: strides must be multiples of 8 elements", __func__);
+    REQUIRE_PTR(q);
+    REQUIRE_PTR(k_cache);
+    REQUIRE_PTR(v_cache);
+    REQUIRE_WORDS(table);
+    REQUIRE_WORDS(lengths);
+    REQUIRE_PTR(out);
+    OPTIONAL_PTR(workspace);
+    const int each = B < escha::kAttendMaxBatch ? B : escha::kAttendMaxBatch;
+    const escha::AttendShape s = escha::attend_shape(each, H, group, D, W, lp, device_sms());
+    REQUIRE(((static_cast<long long>(W) << lp) / escha::kAttendBlock + 1) * each * H * s.chunks <
+                0x7fffffffll,
+            "%s: %d requests of up to %lld tokens and %d heads are more than one launch numbers",
+            __func__, each, static_cast<long long>(W) << lp, H);
+    const size_t need = s.meta_bytes + s.ml_bytes + s.part_bytes;
+    REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
+            "%s: workspace of %zu bytes, %zu needed", __func__, workspace ? workspace_bytes : 0, need);
+    escha::AttendParams p{};
+    p.q_row = q_row; p.q_head = q_head;
+    p.k_cache = k_cache; p.v_cache = v_cache; p.k_scale = k_scale; p.v_scale = v_scale;
+    if (need != 0) {
+        char* w = static_cast<char*>(workspace);
+        p.meta = reinterpret_cast<int32_t*>(w);
+        p.part_ml = reinterpret_cast<float*>(w + s.meta_bytes);
+        p.part = reinterpret_cast<float*>(w + s.meta_bytes + s.ml_bytes);
+    }
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.H = H; p.group = group; p.chunks = s.chunks; p.heads = s.heads; p.D = D; p.W = W;
+    p.log_page = lp; p.n_pages = n_pages;
+    // larger batches take one launch after the other (each waits for the one before, so they
+    // share the workspace)
+    for (int b = 0; b < B; b += each) {
+        p.B = B - b < each ? B - b : each;
+        p.ctas = escha::attend_shape(p.B, H, group, D, W, lp, device_sms()).ctas;
+        p.q = static_cast<const char*>(q) + 2ll * b * q_row;
+        p.out = static_cast<char*>(out) + 2ll * b * H * group * D;
+        p.table = table + static_cast<long long>(b) * W;
+        p.lengths = lengths + b;
+        const cudaError_t e = escha::launch_attend(p, q_type, cache_type, s.split, as_stream(stream));
+        if (e != cudaSuccess) return cuda_result(e, "escha_paged_attend");
+    }
+    return ESCHA_OK;
 }
 
 }  // extern "C"

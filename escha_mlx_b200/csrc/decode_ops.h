@@ -1,0 +1,77 @@
+// Launchers of the decode step's operators around the projections: page plans, the paged
+// key-value cache, attention over it and sampling.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace escha {
+
+// Element types of the boundary (escha_b200.h: ESCHA_F16 ...).
+constexpr int kF16 = 0, kBF16 = 1, kF32 = 2, kI8 = 3;
+
+constexpr int kPlanMaxBatch = 4096;
+
+struct PlanParams {
+    int32_t* table;          // [B, W], entries of newly taken pages are written
+    const int32_t* lengths;  // [B]
+    const int32_t* added;    // [B]
+    const int32_t* free_pages;  // [F]
+    const int32_t* head;     // [1]
+    int32_t* slots;          // [rows]
+    int32_t* positions;      // [rows]
+    int32_t* starts;         // [B + 1]
+    int32_t* ends;           // [B]
+    int32_t* head_out;       // [1]
+    int32_t* refused;        // [1]
+    int B, W, F, rows, log_page, n_pages;
+};
+cudaError_t launch_page_plan(const PlanParams& p, cudaStream_t st);
+
+struct AppendParams {
+    const void* k;           // [T, H, D] with strides (elements)
+    const void* v;
+    long k_row, k_head, v_row, v_head;
+    const int32_t* slots;    // [T]
+    void* k_cache;           // [n_pages, H, P, D]
+    void* v_cache;
+    float* k_scale;          // [n_pages, H, P], 8-bit cache only
+    float* v_scale;
+    int T, H, D, log_page, n_pages;
+};
+// 16-bit caches take rows of their own type (a copy); the 8-bit cache takes f16 or bf16 rows.
+cudaError_t launch_paged_append(const AppendParams& p, int in_type, int cache_type, cudaStream_t st);
+
+// Requests of one attention launch (their prefix of token blocks sits in shared memory).
+constexpr int kAttendMaxBatch = 1024;
+// Tokens that a CTA takes at a time, and the granularity of the split over the cache.
+constexpr int kAttendBlock = 64;
+
+struct AttendParams {
+    const void* q;           // [B, H * group, D] with strides (elements)
+    long q_row, q_head;
+    const void* k_cache;     // [n_pages, H, P, D]
+    const void* v_cache;
+    const float* k_scale;    // [n_pages, H, P], 8-bit cache only
+    const float* v_scale;
+    const int32_t* table;    // [B, W]
+    const int32_t* lengths;  // [B]
+    void* out;               // [B, H * group, D]
+    int32_t* meta;           // [ctas][2]: row that a CTA starts and leaves unfinished, last CTA of it
+    float* part_ml;          // [2 * ctas][heads][2]
+    float* part;             // [2 * ctas][heads][D]
+    float scale_log2;        // score scale times log2(e)
+    int B, H, group, chunks, heads, D, W, log_page, n_pages, ctas;
+};
+struct AttendShape {
+    int heads;    // query heads of one work item: 8 or 16 at most
+    int chunks;   // work items per key/value head
+    int ctas;     // CTAs of the launch
+    bool split;   // whether a row may be cut between CTAs at all
+    size_t meta_bytes, ml_bytes, part_bytes;
+};
+AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, int sms);
+cudaError_t launch_attend(const AttendParams& p, int q_type, int cache_type, bool split,
+                          cudaStream_t st);
+
+}  // namespace escha

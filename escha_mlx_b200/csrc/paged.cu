@@ -1,0 +1,283 @@
+// Page plans and stores of the paged key-value cache.
+//
+// Plan.  With page size P, request b holds have_b = ceil(len_b / P) pages and needs
+// then_b = ceil((len_b + new_b) / P) after the step.  Rows of the step are packed by request
+// (first_b = exclusive prefix of new), missing pages are taken from the free list in request
+// order (before_b = exclusive prefix of then - have).  Everything follows from two prefix
+// sums over the batch, so every CTA computes both for itself (a batch is a few KB, read from
+// L2) and then writes its share of the rows and table entries: one launch, no wait between
+// CTAs, no counters.  Bound by launch and load latency, not by its bytes.
+//
+// Store.  One thread per 8 elements of a row; a copy for 16-bit caches.  The 8-bit cache
+// keeps, per token and head, scale = max|x| / 127 in 32 bits and the code nearest to
+// x / scale: the D/8 threads of a row find the maximum by shuffles.  Bound by HBM.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdlib>
+#include <cstring>
+#include <utility>
+
+#include "common.cuh"
+#include "decode_ops.h"
+
+namespace escha {
+namespace {
+
+constexpr int kPlanThreads = 256;
+
+// Exclusive prefix of one value per thread over the block, and the block's sum.
+__device__ __forceinline__ long long block_exclusive(long long v, long long* total) {
+    __shared__ long long sums[kPlanThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
+    }
+    __syncthreads();          // the previous use of sums is over
+    if (lane == 31) sums[warp] = inc;
+    __syncthreads();
+    long long base = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+        if (w < warp) base += sums[w];
+        all += sums[w];
+    }
+    *total = all;
+    return base + inc - v;
+}
+
+// Last index b in [0, n) with prefix[b] <= x (prefix[0] == 0 <= x).
+__device__ __forceinline__ int owner_of(const int* prefix, int n, int x) {
+    int lo = 0, hi = n;       // prefix[lo] <= x, prefix[hi] > x or hi == n
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+struct Request {
+    long long len, add;
+    int have, need;
+    bool valid;
+};
+__device__ __forceinline__ Request request(const PlanParams& p, int b, long long first) {
+    Request r;
+    r.len = p.lengths[b];
+    r.add = p.added[b];
+    const long long most = static_cast<long long>(p.W) << p.log_page;
+    r.valid = r.len >= 0 && r.add >= 0 && r.len + r.add <= most && first + r.add <= p.rows;
+    const long long up = (1ll << p.log_page) - 1;
+    r.have = r.valid ? static_cast<int>((r.len + up) >> p.log_page) : 0;
+    r.need = r.valid ? static_cast<int>((r.len + r.add + up) >> p.log_page) - r.have : 0;
+    return r;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParams p) {
+    __shared__ int s_first[kPlanMaxBatch];    // first row of a request
+    __shared__ int s_before[kPlanMaxBatch];   // pages taken before it
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int tid = threadIdx.x;
+    const int each = (p.B + kPlanThreads - 1) / kPlanThreads;
+    const int lo = min(tid * each, p.B), hi = min(lo + each, p.B);
+    const bool writes = blockIdx.x == 0;
+
+    long long sum = 0, rows_in;
+    for (int b = lo; b < hi; ++b) sum += max(p.added[b], 0);
+    long long at = block_exclusive(sum, &rows_in);
+    const long long first0 = at;
+    long long need = 0, pages_in;
+    for (int b = lo; b < hi; ++b) {
+        s_first[b] = static_cast<int>(min(at, 0x7fffffffll));
+        if (writes) p.starts[b] = s_first[b];
+        need += request(p, b, at).need;
+        at += max(p.added[b], 0);
+    }
+    long long before = block_exclusive(need, &pages_in);
+    // the list from head on; a head outside the list leaves nothing to take
+    const int head = *p.head;
+    const long long avail = head >= 0 && head <= p.F ? p.F - head : 0;
+    long long took = 0, refused = 0;
+    at = first0;
+    for (int b = lo; b < hi; ++b) {
+        const Request r = request(p, b, at);
+        s_before[b] = static_cast<int>(before);
+        const bool fine = r.valid && (r.need == 0 || before + r.need <= avail);
+        took += fine ? r.need : 0;
+        refused += !fine;
+        if (writes) {
+            const long long most = static_cast<long long>(p.W) << p.log_page;
+            p.ends[b] = static_cast<int>(fine ? r.len + r.add : min(max(r.len, 0ll), most));
+        }
+        before += r.need;
+        at += max(p.added[b], 0);
+    }
+    long long all_took, all_refused;
+    block_exclusive(took, &all_took);
+    block_exclusive(refused, &all_refused);      // its barriers also publish s_first, s_before
+    if (writes && tid == 0) {
+        p.starts[p.B] = static_cast<int>(min(rows_in, 0x7fffffffll));
+        *p.head_out = head + static_cast<int>(all_took);
+        *p.refused = static_cast<int>(all_refused);
+    }
+    const int step = gridDim.x * kPlanThreads, me = blockIdx.x * kPlanThreads + tid;
+    // Requests are served in order until the list ends, so the pages taken are the first
+    // all_took of the prefix: page i belongs to the request whose range holds it.
+    for (int i = me; i < all_took; i += step) {
+        const int b = owner_of(s_before, p.B, i);
+        const Request r = request(p, b, s_first[b]);
+        p.table[static_cast<size_t>(b) * p.W + r.have + (i - s_before[b])] = p.free_pages[head + i];
+    }
+    for (int row = me; row < p.rows; row += step) {
+        int slot = -1, pos = 0;
+        if (row < rows_in) {
+            const int b = owner_of(s_first, p.B, row);
+            const Request r = request(p, b, s_first[b]);
+            if (r.valid && (r.need == 0 || s_before[b] + static_cast<long long>(r.need) <= avail)) {
+                pos = static_cast<int>(r.len) + row - s_first[b];
+                const int idx = pos >> p.log_page;
+                // pages that the request already held are in its table; the others are read
+                // from the list, since another CTA may be writing their entries now
+                const int page = idx < r.have ? p.table[static_cast<size_t>(b) * p.W + idx]
+                                              : p.free_pages[head + s_before[b] + idx - r.have];
+                if (page >= 0 && page < p.n_pages)
+                    slot = (page << p.log_page) + (pos & ((1 << p.log_page) - 1));
+            }
+        }
+        p.slots[row] = slot;
+        p.positions[row] = pos;
+    }
+}
+
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    static __device__ float2 f32(uint32_t w) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    }
+};
+template <> struct Pair<__nv_bfloat16> {
+    static __device__ float2 f32(uint32_t w) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+};
+
+// The code nearest to x / scale, ties to even.  The rounded quotient can land on the wrong
+// side of a middle; its remainder x - code * scale (one rounding, by FMA) tells.
+__device__ __forceinline__ int code_of(float x, float scale) {
+    float c = rintf(__fdiv_rn(x, scale));
+    const float r = __fmaf_rn(-c, scale, x), half = 0.5f * scale;
+    if (r > half) c += 1.0f;
+    else if (r < -half) c -= 1.0f;
+    return static_cast<int>(fminf(fmaxf(c, -127.0f), 127.0f));
+}
+
+constexpr int kAppendThreads = 256;
+
+// T: type of the rows; Q: 8-bit cache.  Item = 8 elements of one row of one head of k or v.
+template <typename T, bool Q>
+__global__ void __launch_bounds__(kAppendThreads)
+paged_append_kernel(const AppendParams p, int log_d8) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int d8 = 1 << log_d8;                           // items per row of a head: 8, 16 or 32
+    const long items = 2l * p.T * p.H * d8;               // [T][k, v][H][D / 8]
+    const long step = static_cast<long>(gridDim.x) * kAppendThreads;
+    // every thread of a warp runs the same rounds (items are whole rows of 8..32 threads and
+    // a warp's first item is a multiple of 32), so the shuffles below always meet
+    for (long i0 = static_cast<long>(blockIdx.x) * kAppendThreads + (threadIdx.x & ~31); i0 < items;
+         i0 += step) {
+        const long i = i0 + (threadIdx.x & 31);
+        const bool in = i < items;
+        const int d = static_cast<int>(i & (d8 - 1));
+        const long hh = i >> log_d8;                      // [T][k, v][H]
+        const int h = static_cast<int>(hh % p.H);
+        const long tv = hh / p.H;
+        const bool is_v = tv & 1;
+        const long row = tv >> 1;
+        const int slot = in ? p.slots[row] : -1;
+        const bool stored = slot >= 0 && (slot >> p.log_page) < p.n_pages;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (stored) {
+            const T* src = is_v ? static_cast<const T*>(p.v) + row * p.v_row + h * p.v_head
+                                : static_cast<const T*>(p.k) + row * p.k_row + h * p.k_head;
+            x = *reinterpret_cast<const uint4*>(src + d * 8);
+        }
+        const long page = slot >> p.log_page;
+        const long at = ((page * p.H + h) << p.log_page) + (slot & ((1 << p.log_page) - 1));
+        if constexpr (!Q) {
+            if (stored) {
+                T* dst = static_cast<T*>(is_v ? p.v_cache : p.k_cache) + at * p.D + d * 8;
+                *reinterpret_cast<uint4*>(dst) = x;
+            }
+        } else {
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            float f[8];
+            float top = 0.0f;
+            bool odd = false;                             // NaN or infinite
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 y = Pair<T>::f32(w[k]);
+                f[2 * k] = y.x;
+                f[2 * k + 1] = y.y;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                top = fmaxf(top, fabsf(f[k]));
+                odd |= !(fabsf(f[k]) <= 3.4e38f);
+            }
+            if (odd) top = __int_as_float(0x7f800000);
+            for (int o = d8 >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // a row that is not finite is stored as NaN: its values have no scale
+            const bool finite = top <= 3.4e38f;
+            const float scale = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fc00000);
+            if (stored) {
+                uint32_t c[2] = {0, 0};
+                if (finite && scale > 0.0f) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        c[k >> 2] |= (static_cast<uint32_t>(code_of(f[k], scale)) & 0xffu)
+                                     << (8 * (k & 3));
+                }
+                int8_t* dst = static_cast<int8_t*>(is_v ? p.v_cache : p.k_cache) + at * p.D + d * 8;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+                if (d == 0) (is_v ? p.v_scale : p.k_scale)[at] = scale;
+            }
+        }
+    }
+}
+
+int sm_count() {
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return sms;
+}
+
+}  // namespace
+
+cudaError_t launch_page_plan(const PlanParams& p, cudaStream_t st) {
+    const int most = (p.rows + kPlanThreads - 1) / kPlanThreads;
+    const int grid = most < 1 ? 1 : most > sm_count() ? sm_count() : most;
+    return launch_chained(page_plan_kernel, dim3(grid), dim3(kPlanThreads), 0, st, p);
+}
+
+cudaError_t launch_paged_append(const AppendParams& p, int in_type, int cache_type, cudaStream_t st) {
+    const int log_d8 = p.D == 64 ? 3 : p.D == 128 ? 4 : 5;
+    const long items = 2l * p.T * p.H << log_d8;
+    const long most = (items + kAppendThreads - 1) / kAppendThreads;
+    const long cap = 8l * sm_count();
+    const dim3 grid(static_cast<unsigned>(most < cap ? most : cap));
+    if (cache_type == kI8)
+        return in_type == kF16
+                   ? launch_chained(paged_append_kernel<__half, true>, grid, dim3(kAppendThreads), 0, st, p, log_d8)
+                   : launch_chained(paged_append_kernel<__nv_bfloat16, true>, grid, dim3(kAppendThreads), 0, st, p, log_d8);
+    // a 16-bit copy: the type does not matter
+    return launch_chained(paged_append_kernel<__half, false>, grid, dim3(kAppendThreads), 0, st, p, log_d8);
+}
+
+}  // namespace escha

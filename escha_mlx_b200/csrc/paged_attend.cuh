@@ -1,0 +1,705 @@
+// Attention of one new token per request over the paged key-value cache.
+//
+//   S = scale * q K^T over the request's tokens,  P = softmax(S),  O = P V
+//
+// per query head; the `group` query heads of a key/value head read the same K and V, so they
+// are the columns of one product and the cache is read once.  Bound by reading the cache from
+// HBM: at 8 query heads a byte of it meets 8 multiply-adds, far below what even mma.sync
+// offers, and a token block of 16 x 8 heads is no tile for tcgen05 (128 rows at least).
+//
+// Layout.  Both products are computed transposed, S^T = K q^T and O^T = V^T P^T, so that the
+// cache is the A operand (16 tokens, resp. 16 channels, per mma.m16n8k16) and the heads are
+// the 8 columns.  The order of the summed index is free, so lane (g, t) = (lane / 4, lane % 4)
+// takes 16 contiguous bytes of token rows g and g + 8 for the first product, and contiguous
+// bytes of token rows 2t, 2t + 1, 2t + 8, 2t + 9 for the second, whose pairs along the tokens
+// are put together by byte permutes.  Every lane reads from shared memory exactly the bytes
+// that it brought there with its own cp.async: no bank conflicts, no barriers and no
+// warp-level waits in the loop, and rows past a request's end are zero-filled, never read.
+// Each warp has a ring of its own (key tile, value tile, key tile, ... of 16 tokens).
+//
+// Softmax.  Scores are held in 32 bits, times log2(e); a running maximum per head, sums in
+// 32 bits per lane until the end.  P is rounded to 16 bits for the product, as a pair hi + lo
+// of them, so that this rounding stays below that of the output; with binary16 P is scaled by
+// 2^13 against underflow of the many small weights of a long context.  The 8-bit cache holds
+// codes, exact in binary16; K's scale multiplies the score, V's the weight (the running
+// maximum then includes V's exponent, so that the weights stay in range).
+//
+// Split.  The work is a line of blocks of 64 tokens, over all requests and key/value heads;
+// each CTA takes an equal share of it, whatever the lengths are, and cuts rows where its share
+// ends.  A CTA leaves at most two unfinished rows (its first and its last); a second, chained
+// kernel joins the pieces of each row in order.  No counters, nothing to clear.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdlib>
+#include <cstring>
+#include <utility>
+
+#include "common.cuh"
+#include "decode_ops.h"
+#include "kernels.h"
+
+namespace escha {
+namespace attend {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = 16;
+static_assert(kTile * kWarps == kAttendBlock, "a block is one tile per warp");
+
+// Copies of one lane, completed by cp.async.wait_group; bytes past `have` are zero-filled.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int have) {
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(have), "n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <bool BF>
+__device__ __forceinline__ void mma(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
+    if constexpr (!BF) {
+        mma16816(d, a0, a1, a2, a3, b0, b1);
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (!BF) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (!BF) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// Codes of an 8-bit word, offset to 0..255: byte pairs (0, 1) or (2, 3) as binary16.  0x6400 | u
+// is 1024 + u; minus 1152 is the code, exactly.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t offset_word) {
+    const uint32_t x = __byte_perm(offset_word, 0x64646464u, SEL);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+template <int BYTES> struct Words;
+template <> struct Words<16> { uint4 v; __device__ uint32_t operator[](int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; } };
+template <> struct Words<8> { uint2 v; __device__ uint32_t operator[](int i) const { return i == 0 ? v.x : v.y; } };
+template <> struct Words<4> { uint32_t v; __device__ uint32_t operator[](int) const { return v; } };
+
+// QBF: queries and output are bfloat16.  I8: 8-bit cache.  D: channels of a head.
+// NT: groups of 8 query heads.
+template <bool QBF, bool I8, int D, int NT>
+struct Shape {
+    static constexpr bool kBF = QBF && !I8;               // type of the products
+    static constexpr int kElem = I8 ? 1 : 2;
+    static constexpr int kRow = D * kElem;                // bytes of a token's row
+    static constexpr int kChunks = kRow / 64;             // 64-byte pieces of a row
+    static constexpr int kHalf = kTile * kRow;            // bytes of a key or value tile
+    // depth of a warp's ring: two or three tiles ahead, whatever their size
+    static constexpr int kStages = kHalf >= 8192 ? 3 : kHalf >= 4096 ? (I8 ? 5 : 6) : 8;
+    static constexpr int kSets = kRow == 512 ? 2 : 1;     // value rows as 16 pieces per set
+    static constexpr int kPiece = kRow / kSets / 16;      // bytes of a piece: 16, 8 or 4
+    static constexpr int kPerPiece = kPiece / kElem;      // channels of a piece
+    static constexpr int kMma = kSets * kPerPiece;        // O^T tiles of 16 channels
+    static constexpr int kScales = I8 ? 4 * 32 * 4 : 0;   // bytes of a tile's scales in the ring
+    static constexpr int kQWords = I8 ? 8 : 4;            // query words per lane and chunk
+    static constexpr int kQBytes = NT * kChunks * kQWords * 4 * 32;
+    static constexpr int kRingStage = kHalf + kScales;
+    static constexpr int kRing = kWarps * kStages * kRingStage;
+    static constexpr int kHeads = 8 * NT;
+    static constexpr int kJoin = kWarps * kHeads * (D + 4) * 4;   // the warps' sums, over the ring
+    static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
+    static constexpr int kFixed = (kAttendMaxBatch + 4) * 4 + 2 * kWarps * kHeads * 4 + kHeads * 4 + 64;
+    static constexpr int kShared = kBody + kQBytes + kFixed;
+};
+
+// Exclusive prefix of the requests' block counts in s_prefix[0 .. B], by the whole CTA.
+__device__ __forceinline__ void block_counts(const AttendParams& p, int* s_prefix, int* s_sums) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kEach = kAttendMaxBatch / kThreads;
+    const int most = p.W << p.log_page;
+    int n[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int b = tid * kEach + i;
+        const int len = b < p.B ? min(max(p.lengths[b], 0), most) : 0;
+        n[i] = (len + kAttendBlock - 1) / kAttendBlock;
+        sum += n[i];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
+    }
+    if (lane == 31) s_sums[warp] = inc;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < warp; ++w) at += s_sums[w];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int b = tid * kEach + i;
+        if (b <= p.B) s_prefix[b] = at;
+        at += n[i];
+    }
+    if (tid == kThreads - 1 && p.B == kAttendMaxBatch) s_prefix[p.B] = at;
+    __syncthreads();
+}
+
+template <bool QBF, bool I8, int D, int NT>
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p) {
+    using S = Shape<QBF, I8, D, NT>;
+    constexpr bool BF = S::kBF;
+    // power of two on the weights (binary16 products only)
+    constexpr float kLift = BF ? 0.0f : 13.0f;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t* s_body = smem;
+    uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + S::kBody);
+    int* s_prefix = reinterpret_cast<int*>(smem + S::kBody + S::kQBytes);
+    float* s_m = reinterpret_cast<float*>(s_prefix + kAttendMaxBatch + 4);
+    float* s_l = s_m + kWarps * S::kHeads;
+    float* s_qscale = s_l + kWarps * S::kHeads;
+    int* s_sums = reinterpret_cast<int*>(s_qscale + S::kHeads);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    block_counts(p, s_prefix, s_sums);
+
+    const int per_request = p.H * p.chunks;               // rows of a request
+    const long long total = static_cast<long long>(s_prefix[p.B]) * per_request;
+    const int c = blockIdx.x;
+    // as many CTAs as there are blocks at most, so that no share is empty
+    const long long shares = min(static_cast<long long>(p.ctas), total);
+    long long u = c < shares ? total * c / shares : 0;
+    const long long u_end = c < shares ? total * (c + 1) / shares : 0;
+    using QT = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
+    const QT* q = static_cast<const QT*>(p.q);
+    QT* out = static_cast<QT*>(p.out);
+    const int heads_total = p.H * p.group;
+
+    // requests without a token: zeros
+    for (int b = c; b < p.B; b += p.ctas)
+        if (s_prefix[b + 1] == s_prefix[b])
+            for (int i = tid; i < heads_total * D / 8; i += kThreads)
+                reinterpret_cast<uint4*>(out + static_cast<size_t>(b) * heads_total * D)[i] =
+                    make_uint4(0, 0, 0, 0);
+    int unfinished_row = -1, unfinished_last = -1;
+
+    const uint32_t ring = smem_u32(s_body) + warp * (S::kStages * S::kRingStage);
+    const uint8_t* ring_ptr = s_body + warp * (S::kStages * S::kRingStage);
+    const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache);
+    const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
+
+    while (u < u_end) {
+        // the row that holds block u
+        int lo = 0, hi = p.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (static_cast<long long>(s_prefix[mid]) * per_request <= u) lo = mid; else hi = mid;
+        }
+        const int b = lo;
+        const int blocks = s_prefix[b + 1] - s_prefix[b];
+        const int in_request = static_cast<int>(u - static_cast<long long>(s_prefix[b]) * per_request);
+        const int rr = in_request / blocks;               // head and chunk
+        const int k0 = in_request - rr * blocks;
+        const int k1 = static_cast<int>(min(static_cast<long long>(blocks), k0 + (u_end - u)));
+        const int h = rr / p.chunks, chunk = rr - h * p.chunks;
+        const int head0 = h * p.group + chunk * S::kHeads;
+        const int nheads = min(S::kHeads, p.group - chunk * S::kHeads);
+        const int len = min(max(p.lengths[b], 0), p.W << p.log_page);
+        const int t0 = k0 * kAttendBlock, t1 = min(len, k1 * kAttendBlock);
+        const bool starts = k0 == 0, ends = k1 == blocks;
+        const int32_t* pages = p.table + static_cast<size_t>(b) * p.W;
+
+        // tiles of this warp: warp, warp + kWarps, ... of the segment
+        const int tiles = (t1 - t0 + kTile - 1) / kTile;
+        const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+        const int halves = 2 * mine;                      // K0, V0, K1, V1, ...
+        int ids = -1;                                     // lane j: page of tile j (mod 32)
+        uint32_t bad = 0;                                 // tiles (mod 32) without a usable page
+        const uint8_t *k_src = kc, *v_src = vc;           // first token of the tile being fetched
+        const float *ks_src = p.k_scale, *vs_src = p.v_scale;
+        int k_have = 0;                                   // its tokens
+        auto fetch = [&](int i, int stage) {
+            if (i < halves) {
+                const int j = i >> 1;
+                const uint32_t dst = ring + stage * S::kRingStage;
+                if ((i & 1) == 0) {
+                    if ((j & 31) == 0) {
+                        const int tok = t0 + kTile * (warp + kWarps * (j + lane));
+                        ids = tok < t1 ? pages[tok >> p.log_page] : -1;
+                    }
+                    const int page = __shfl_sync(0xffffffffu, ids, j & 31);
+                    const int tok = t0 + kTile * (warp + kWarps * j);
+                    const bool ok = page >= 0 && page < p.n_pages;
+                    bad = (bad & ~(1u << (j & 31))) | (ok ? 0u : 1u << (j & 31));
+                    k_have = ok ? min(kTile, t1 - tok) : 0;
+                    const size_t row = (((ok ? static_cast<size_t>(page) : 0) * p.H + h) << p.log_page) +
+                                       (tok & ((1 << p.log_page) - 1));
+                    k_src = kc + row * S::kRow;
+                    v_src = vc + row * S::kRow;
+                    if constexpr (I8) {
+                        ks_src = p.k_scale + row;
+                        vs_src = p.v_scale + row;
+                    }
+                    const bool in0 = g < k_have, in1 = g + 8 < k_have;
+                    const uint8_t* r0 = k_src + (in0 ? g * S::kRow : 0) + t * 16;
+                    const uint8_t* r1 = k_src + (in1 ? (g + 8) * S::kRow : 0) + t * 16;
+#pragma unroll
+                    for (int x = 0; x < S::kChunks; ++x) {
+                        copy_async<16>(dst + (2 * x * 32 + lane) * 16, r0 + x * 64, in0 ? 16 : 0);
+                        copy_async<16>(dst + ((2 * x + 1) * 32 + lane) * 16, r1 + x * 64, in1 ? 16 : 0);
+                    }
+                    if constexpr (I8) {
+                        const uint32_t sd = dst + S::kHalf + lane * 16;
+                        copy_async<4>(sd, ks_src + (in0 ? g : 0), in0 ? 4 : 0);
+                        copy_async<4>(sd + 4, ks_src + (in1 ? g + 8 : 0), in1 ? 4 : 0);
+                        copy_async<4>(sd + 8, vs_src + (in0 ? g : 0), in0 ? 4 : 0);
+                        copy_async<4>(sd + 12, vs_src + (in1 ? g + 8 : 0), in1 ? 4 : 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int r = 2 * t + (y & 1) + (y >> 1) * 8;
+                        const bool in = r < k_have;
+                        const uint8_t* src = v_src + (in ? r * S::kRow : 0) + g * S::kPiece;
+#pragma unroll
+                        for (int z = 0; z < 2 * S::kSets; ++z)
+                            copy_async<S::kPiece>(dst + ((z * 4 + y) * 32 + lane) * S::kPiece,
+                                                  src + z * 8 * S::kPiece, in ? S::kPiece : 0);
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+        __syncthreads();      // the previous row's sums (in the ring) and queries are read
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) fetch(i, i);
+
+        // queries of the row: lane (g, t) of chunk x holds head g's channels that meet the
+        // lane's bytes of the key rows
+        if (warp < NT) {
+            const int nt = warp;
+            const bool in = nt * 8 + g < nheads;
+            const QT* src = q + static_cast<long>(b) * p.q_row +
+                            static_cast<long>(head0 + (in ? nt * 8 + g : 0)) * p.q_head;
+            uint4 w[S::kChunks * S::kQWords / 4];
+#pragma unroll
+            for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
+                // 16 channels (8-bit cache) are two loads of 8
+                const int off = I8 ? (x >> 1) * 64 + t * 16 + (x & 1) * 8 : x * 32 + t * 8;
+                w[x] = in ? *reinterpret_cast<const uint4*>(src + off) : make_uint4(0, 0, 0, 0);
+            }
+            float by = p.scale_log2;
+            if constexpr (I8 && QBF) {
+                // bfloat16 queries against codes in binary16: bring the row's largest value
+                // to [1, 2) by a power of two
+                float top = 0.0f;
+#pragma unroll
+                for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = unpack2<true>(k == 0 ? w[x].x : k == 1 ? w[x].y : k == 2 ? w[x].z : w[x].w);
+                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 120);
+                const float down = __int_as_float((127 - e) << 23);
+                by *= __int_as_float((127 + e) << 23);
+#pragma unroll
+                for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
+                    uint32_t* v = &w[x].x;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = unpack2<true>(v[k]);
+                        v[k] = pack2<false>(f.x * down, f.y * down);
+                    }
+                }
+            }
+            if (t == 0) s_qscale[nt * 8 + g] = by;
+#pragma unroll
+            for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
+                reinterpret_cast<uint4*>(s_q)[(nt * (S::kChunks * S::kQWords / 4) + x) * 32 + lane] = w[x];
+        }
+        __syncthreads();
+        float qs[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            qs[nt][0] = s_qscale[nt * 8 + 2 * t];
+            qs[nt][1] = s_qscale[nt * 8 + 2 * t + 1];
+        }
+
+        float acc[NT][S::kMma][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int k = 0; k < S::kMma; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][k][e] = 0.0f;
+            m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
+            l[nt][0] = l[nt][1] = 0.0f;
+        }
+
+        int rd = 0, wr = S::kStages - 1;                  // stages to read and to fill next
+        for (int j = 0; j < mine; ++j) {
+            // ---- scores of 16 tokens
+            cp_async_wait<S::kStages - 2>();
+            const uint8_t* tile = ring_ptr + rd * S::kRingStage;
+            float s[NT][4], s2[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < S::kChunks; ++x) {
+                Words<16> r0, r1;
+                r0.v = reinterpret_cast<const uint4*>(tile)[2 * x * 32 + lane];
+                r1.v = reinterpret_cast<const uint4*>(tile)[(2 * x + 1) * 32 + lane];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    Words<16> qa, qb;
+                    constexpr int kPer = S::kQWords / 4;
+                    qa.v = reinterpret_cast<const uint4*>(s_q)[((nt * S::kChunks + x) * kPer) * 32 + lane];
+                    if constexpr (!I8) {
+                        mma<BF>(s[nt], r0[0], r1[0], r0[1], r1[1], qa[0], qa[1]);
+                        mma<BF>(s2[nt], r0[2], r1[2], r0[3], r1[3], qa[2], qa[3]);
+                    } else {
+                        qb.v = reinterpret_cast<const uint4*>(s_q)[((nt * S::kChunks + x) * kPer + 1) * 32 + lane];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t a = r0[k] ^ 0x80808080u, e = r1[k] ^ 0x80808080u;
+                            mma<false>(k & 1 ? s2[nt] : s[nt], codes_f16<0x4140>(a), codes_f16<0x4140>(e),
+                                       codes_f16<0x4342>(a), codes_f16<0x4342>(e),
+                                       k < 2 ? qa[2 * k] : qb[2 * k - 4], k < 2 ? qa[2 * k + 1] : qb[2 * k - 3]);
+                        }
+                    }
+                }
+            }
+            float4 sc = make_float4(1.0f, 1.0f, 1.0f, 1.0f);   // K's, then V's scales of tokens g, g + 8
+            if constexpr (I8) sc = reinterpret_cast<const float4*>(tile + S::kHalf)[lane];
+            fetch(2 * j + S::kStages - 1, wr);
+            rd = rd + 1 == S::kStages ? 0 : rd + 1;
+            wr = wr + 1 == S::kStages ? 0 : wr + 1;
+
+            // ---- weights
+            const int tok = t0 + kTile * (warp + kWarps * j);
+            const int have = (bad >> (j & 31)) & 1 ? 0 : min(kTile, t1 - tok);
+            uint32_t hi0[NT], hi1[NT], lo0[NT], lo1[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float y = s[nt][e] + s2[nt][e];
+                    if constexpr (I8) y *= e < 2 ? sc.x : sc.y;
+                    y *= qs[nt][e & 1];
+                    x[e] = g + (e < 2 ? 0 : 8) < have ? y : __int_as_float(0xff800000);
+                }
+                float up[2];
+                if constexpr (I8) {
+                    // exponents of V's scales, so that weight times scale stays at most 2
+                    const float e0 = static_cast<float>(max((__float_as_int(sc.z) >> 23) - 127, -90));
+                    const float e1 = static_cast<float>(max((__float_as_int(sc.w) >> 23) - 127, -90));
+                    up[0] = fmaxf(x[0] + e0, x[2] + e1);
+                    up[1] = fmaxf(x[1] + e0, x[3] + e1);
+                } else {
+                    up[0] = fmaxf(x[0], x[2]);
+                    up[1] = fmaxf(x[1], x[3]);
+                }
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    up[0] = fmaxf(up[0], __shfl_xor_sync(0xffffffffu, up[0], d));
+                    up[1] = fmaxf(up[1], __shfl_xor_sync(0xffffffffu, up[1], d));
+                }
+                const bool raise = up[0] > m[nt][0] || up[1] > m[nt][1];
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float to = fmaxf(m[nt][e], up[e]);
+                        const float a = to == __int_as_float(0xff800000) ? 1.0f : exp2_approx(m[nt][e] - to);
+                        m[nt][e] = to;
+                        l[nt][e] *= a;
+#pragma unroll
+                        for (int k = 0; k < S::kMma; ++k) {
+                            acc[nt][k][e] *= a;
+                            acc[nt][k][e + 2] *= a;
+                        }
+                    }
+                }
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // no finite score yet: every weight of the tile is zero
+                    const float ref = m[nt][e & 1] == __int_as_float(0xff800000) ? 0.0f : m[nt][e & 1] - kLift;
+                    w[e] = exp2_approx(x[e] - ref);
+                    l[nt][e & 1] += w[e];
+                    if constexpr (I8) {
+                        // a masked token's scale is zero-filled: 0 * 0
+                        w[e] *= e < 2 ? sc.z : sc.w;
+                    }
+                }
+                const uint32_t h0 = pack2<BF>(w[0], w[1]), h1 = pack2<BF>(w[2], w[3]);
+                const float2 f0 = unpack2<BF>(h0), f1 = unpack2<BF>(h1);
+                hi0[nt] = transpose8(h0);
+                hi1[nt] = transpose8(h1);
+                lo0[nt] = transpose8(pack2<BF>(w[0] - f0.x, w[1] - f0.y));
+                lo1[nt] = transpose8(pack2<BF>(w[2] - f1.x, w[3] - f1.y));
+            }
+
+            // ---- weighted values
+            cp_async_wait<S::kStages - 2>();
+            tile = ring_ptr + rd * S::kRingStage;
+#pragma unroll
+            for (int z = 0; z < S::kSets; ++z) {
+                Words<S::kPiece> v[2][4];                 // piece g, g + 8; tokens 2t, 2t+1, 2t+8, 2t+9
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                    v[y >> 2][y & 3].v = reinterpret_cast<const decltype(v[0][0].v)*>(tile)[(z * 8 + y) * 32 + lane];
+#pragma unroll
+                for (int w = 0; w < S::kPiece / 4; ++w) {
+                    uint32_t a[4][I8 ? 4 : 2];            // operand registers of the word's channels
+                    if constexpr (!I8) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {     // r: (piece, token pair) in A's order
+                            const uint32_t v0 = v[r & 1][(r >> 1) * 2][w], v1 = v[r & 1][(r >> 1) * 2 + 1][w];
+                            a[r][0] = __byte_perm(v0, v1, 0x5410);
+                            a[r][1] = __byte_perm(v0, v1, 0x7632);
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t v0 = v[r & 1][(r >> 1) * 2][w] ^ 0x80808080u;
+                            const uint32_t v1 = v[r & 1][(r >> 1) * 2 + 1][w] ^ 0x80808080u;
+                            const uint32_t p01 = __byte_perm(v0, v1, 0x5140), p23 = __byte_perm(v0, v1, 0x7362);
+                            a[r][0] = codes_f16<0x4140>(p01);
+                            a[r][1] = codes_f16<0x4342>(p01);
+                            a[r][2] = codes_f16<0x4140>(p23);
+                            a[r][3] = codes_f16<0x4342>(p23);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < (I8 ? 4 : 2); ++i) {
+                        const int k = z * S::kPerPiece + w * (I8 ? 4 : 2) + i;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<BF>(acc[nt][k], a[0][i], a[1][i], a[2][i], a[3][i], hi0[nt], hi1[nt]);
+                            mma<BF>(acc[nt][k], a[0][i], a[1][i], a[2][i], a[3][i], lo0[nt], lo1[nt]);
+                        }
+                    }
+                }
+            }
+            fetch(2 * j + S::kStages, wr);
+            rd = rd + 1 == S::kStages ? 0 : rd + 1;
+            wr = wr + 1 == S::kStages ? 0 : wr + 1;
+        }
+
+        // ---- join the warps through shared memory
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();                                  // every warp is through with its ring
+        float* s_acc = reinterpret_cast<float*>(s_body);  // [warp][head][D + 4]
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int head = nt * 8 + 2 * t + e;
+                float sum = l[nt][e];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                if (g == 0) {
+                    s_m[warp * S::kHeads + head] = m[nt][e];
+                    s_l[warp * S::kHeads + head] = sum;
+                }
+                float* dst = s_acc + (warp * S::kHeads + head) * (D + 4);
+#pragma unroll
+                for (int z = 0; z < S::kSets; ++z)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int k = 0; k < S::kPerPiece; k += 4)
+                            *reinterpret_cast<float4*>(dst + (z * 16 + half * 8 + g) * S::kPerPiece + k) =
+                                make_float4(acc[nt][z * S::kPerPiece + k][2 * half + e],
+                                            acc[nt][z * S::kPerPiece + k + 1][2 * half + e],
+                                            acc[nt][z * S::kPerPiece + k + 2][2 * half + e],
+                                            acc[nt][z * S::kPerPiece + k + 3][2 * half + e]);
+            }
+        __syncthreads();
+        const int slot = starts ? 2 * c + 1 : 2 * c;      // piece of an unfinished row
+        for (int i = tid; i < nheads * (D / 4); i += kThreads) {
+            const int head = i / (D / 4), d = (i % (D / 4)) * 4;
+            float top = s_m[head];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w * S::kHeads + head]);
+            const float ref = top == __int_as_float(0xff800000) ? 0.0f : top;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float a = exp2_approx(s_m[w * S::kHeads + head] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(s_acc + (w * S::kHeads + head) * (D + 4) + d);
+                sum += a * s_l[w * S::kHeads + head];
+                o.x += a * x.x;
+                o.y += a * x.y;
+                o.z += a * x.z;
+                o.w += a * x.w;
+            }
+            if (starts && ends) {
+                // nothing to attend to (no usable page): zeros
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                QT* dst = out + (static_cast<size_t>(b) * heads_total + head0 + head) * D + d;
+                *reinterpret_cast<uint2*>(dst) =
+                    make_uint2(pack2<QBF>(o.x * inv, o.y * inv), pack2<QBF>(o.z * inv, o.w * inv));
+            } else {
+                const size_t at = static_cast<size_t>(slot) * S::kHeads + head;
+                *reinterpret_cast<float4*>(p.part + at * D + d) = o;
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(top, sum);
+            }
+        }
+        if (starts && !ends) {
+            unfinished_row = b * per_request + rr;
+            // last CTA of the row: the one whose share holds the row's last block
+            const long long last = static_cast<long long>(s_prefix[b]) * per_request +
+                                   static_cast<long long>(rr + 1) * blocks - 1;
+            long long cl = last * shares / total;         // near; settled by the shares themselves
+            while (cl + 1 < shares && total * (cl + 1) / shares <= last) ++cl;
+            while (cl > 0 && total * cl / shares > last) --cl;
+            unfinished_last = static_cast<int>(cl);
+        }
+        u += k1 - k0;
+    }
+    if (tid == 0 && p.meta != nullptr) {
+        p.meta[2 * c] = unfinished_row;
+        p.meta[2 * c + 1] = unfinished_last;
+    }
+}
+
+constexpr int kJoinThreads = 256;
+
+// Joins the pieces of the row that CTA blockIdx.x of the attention started and did not
+// finish: its own last piece, then the first pieces of the following CTAs.
+template <bool QBF, int D>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendParams p) {
+    extern __shared__ __align__(16) float s_w[];          // [ctas] weights, then [groups][D] sums
+    __shared__ float s_red[kJoinThreads / 32 + 1];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int first = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+    const int row = p.meta[2 * first];
+    if (row < 0) return;
+    const int n = p.meta[2 * first + 1] - first + 1;
+    const int per_request = p.H * p.chunks;
+    const int b = row / per_request, rr = row - b * per_request;
+    const int h = rr / p.chunks, chunk = rr - h * p.chunks;
+    if (chunk * p.heads + head >= p.group) return;
+    // piece 0 is slot 2 first + 1; piece i is slot 2 (first + i)
+    auto piece = [&](int i) { return static_cast<size_t>(2 * (first + i) + (i == 0)) * p.heads + head; };
+    float top = __int_as_float(0xff800000);
+    for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, p.part_ml[2 * piece(i)]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if ((tid & 31) == 0) s_red[tid >> 5] = top;
+    __syncthreads();
+    top = s_red[0];
+#pragma unroll
+    for (int w = 1; w < kJoinThreads / 32; ++w) top = fmaxf(top, s_red[w]);
+    const float ref = top == __int_as_float(0xff800000) ? 0.0f : top;
+    __syncthreads();
+    float sum = 0.0f;
+    for (int i = tid; i < n; i += kJoinThreads) {
+        const float a = exp2_approx(p.part_ml[2 * piece(i)] - ref);
+        s_w[i] = a;
+        sum += a * p.part_ml[2 * piece(i) + 1];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if ((tid & 31) == 0) s_red[tid >> 5] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) sum += s_red[w];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+
+    constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+    const int grp = tid / kLanes, d = (tid % kLanes) * 4;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = grp; i < n; i += kGroups) {
+        const float a = s_w[i];
+        const float4 x = *reinterpret_cast<const float4*>(p.part + piece(i) * D + d);
+        o.x += a * x.x;
+        o.y += a * x.y;
+        o.z += a * x.z;
+        o.w += a * x.w;
+    }
+    float* s_o = s_w + ((p.ctas + 3) & ~3);
+    *reinterpret_cast<float4*>(s_o + grp * D + d) = o;
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+        for (int k = 1; k < kGroups; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(s_o + k * D + d);
+            o.x += x.x;
+            o.y += x.y;
+            o.z += x.z;
+            o.w += x.w;
+        }
+        using QT = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
+        QT* dst = static_cast<QT*>(p.out) +
+                  (static_cast<size_t>(b) * p.H * p.group + h * p.group + chunk * p.heads + head) * D + d;
+        *reinterpret_cast<uint2*>(dst) =
+            make_uint2(pack2<QBF>(o.x * inv, o.y * inv), pack2<QBF>(o.z * inv, o.w * inv));
+    }
+}
+
+template <bool QBF, bool I8, int D, int NT>
+cudaError_t launch(const AttendParams& p, bool split, cudaStream_t st) {
+    using S = Shape<QBF, I8, D, NT>;
+    static SmemLimit limit;
+    cudaError_t e = limit.ensure(attend_kernel<QBF, I8, D, NT>, S::kShared);
+    if (e != cudaSuccess) return e;
+    e = launch_chained(attend_kernel<QBF, I8, D, NT>, dim3(p.ctas), dim3(kThreads), S::kShared, st, p);
+    if (e != cudaSuccess || !split) return e;
+    const size_t smem = (((p.ctas + 3) & ~3) + kJoinThreads / (D / 4) * D) * sizeof(float);
+    return launch_chained(attend_join_kernel<QBF, D>, dim3(p.ctas, p.heads), dim3(kJoinThreads), smem,
+                          st, p);
+}
+
+template <bool QBF, bool I8>
+cudaError_t launch_any(const AttendParams& p, bool split, cudaStream_t st) {
+    if (p.heads == 8) {
+        if (p.D == 64) return launch<QBF, I8, 64, 1>(p, split, st);
+        if (p.D == 128) return launch<QBF, I8, 128, 1>(p, split, st);
+        return launch<QBF, I8, 256, 1>(p, split, st);
+    }
+    if (p.D == 64) return launch<QBF, I8, 64, 2>(p, split, st);
+    if (p.D == 128) return launch<QBF, I8, 128, 2>(p, split, st);
+    return launch<QBF, I8, 256, 2>(p, split, st);
+}
+
+}  // namespace attend
+}  // namespace escha

@@ -1,0 +1,8 @@
+// bfloat16 queries over a cache of the same type.
+#include "paged_attend.cuh"
+
+namespace escha {
+namespace attend {
+template cudaError_t launch_any<true, false>(const AttendParams&, bool, cudaStream_t);
+}  // namespace attend
+}  // namespace escha

@@ -1,0 +1,8 @@
+// bfloat16 queries over a cache of 8-bit codes.
+#include "paged_attend.cuh"
+
+namespace escha {
+namespace attend {
+template cudaError_t launch_any<true, true>(const AttendParams&, bool, cudaStream_t);
+}  // namespace attend
+}  // namespace escha

@@ -438,6 +438,64 @@ void escha_debug_gemm_tc_stall(int on, unsigned limit);
  * (about two seconds).  Lets a test watch the barrier give up on a peer that never arrives. */
 void escha_debug_peer_poll_limit(unsigned polls);
 
+/* ---- the decode step around the projections: paged key-value cache, attention, sampling.
+ * No counterpart in the reference, whose caches, attention and sampling are mlx-lm's.
+ * These entry points bound-check on the device what depends on data (page ids, slots,
+ * lengths); int32 arrays need 4-byte alignment only. */
+
+#define ESCHA_F16 0
+#define ESCHA_BF16 1
+#define ESCHA_F32 2
+#define ESCHA_I8 3
+
+/* Block table, slots and positions of a step, from the requests' lengths.
+ * Request b holds lengths[b] tokens in the pages of table[b, :] (W entries, page_size tokens
+ * each, a power of two in [16, 256]) and gets added[b] more; the step's rows are packed by
+ * request, rows of them at most.  The pages it lacks are taken from free_pages[*head ..] in
+ * request order and entered in the table.  A request that cannot be served (a negative
+ * number, more tokens than its table holds, rows past `rows`, or not enough free pages for it
+ * and those before it) is refused: nothing is taken for it and its rows get slot -1.
+ *   slots     [rows]   page * page_size + offset of each row's token; -1 for rows of refused
+ *                      requests, rows past the last request's and pages outside [0, n_pages)
+ *   positions [rows]   the row's place in its request; 0 where it has none
+ *   starts    [B + 1]  first row of each request, then the number of rows asked for
+ *   ends      [B]      tokens of each request after the step
+ *   head_out  [1]      *head plus the pages taken;  refused [1] requests refused
+ * 1 <= B <= 4096.  free_pages may be NULL when F == 0, slots and positions when rows == 0.
+ * Outputs must not overlap inputs. */
+int escha_page_plan(int32_t *table, const int32_t *lengths, const int32_t *added,
+                    const int32_t *free_pages, int F, const int32_t *head, int B, int W,
+                    int page_size, int n_pages, int rows, int32_t *slots, int32_t *positions,
+                    int32_t *starts, int32_t *ends, int32_t *head_out, int32_t *refused,
+                    void *stream);
+
+/* Store rows k, v [T, H, D] (strides in elements, multiples of 8; D in {64, 128, 256}) at
+ * their slots of caches [n_pages, H, page_size, D].  cache_type is in_type (binary16 or
+ * bfloat16: a copy) or ESCHA_I8: per token and head scale = max|x| / 127 (f32) and the code
+ * nearest to x / scale; a row that is not finite is stored as NaN (its scale).  Rows whose
+ * slot is negative or past the cache are skipped; slots of one call must differ. */
+int escha_paged_append(const void *k, long k_row, long k_head, const void *v, long v_row,
+                       long v_head, int in_type, const int32_t *slots, int T, int H, int D,
+                       int page_size, int n_pages, void *k_cache, void *v_cache, int cache_type,
+                       float *k_scale, float *v_scale, void *stream);
+
+/* Scratch that escha_paged_attend needs on the current device (0: none).  It needs no
+ * clearing and carries nothing from call to call. */
+size_t escha_paged_attend_workspace_bytes(int B, int H, int group, int D, int W, int page_size);
+
+/* out[b] = softmax(scale * q[b] K_b^T) V_b for one new token per request: q [B, H * group, D]
+ * (strides in elements, multiples of 8), query head i reads key/value head i / group; K_b, V_b
+ * are the first lengths[b] tokens in the pages table[b, :].  Lengths are taken within
+ * [0, W * page_size]; tokens on pages outside [0, n_pages) are not attended to; a request with
+ * nothing to attend to gives zeros.  Slots past a length are never read.  q_type is
+ * ESCHA_F16 or ESCHA_BF16; the cache has the same type or is ESCHA_I8 with its scales.
+ * Scores, softmax and sums are 32-bit.  out [B, H * group, D] in q_type, dense. */
+int escha_paged_attend(const void *q, long q_row, long q_head, int q_type, const void *k_cache,
+                       const void *v_cache, int cache_type, const float *k_scale,
+                       const float *v_scale, const int32_t *table, const int32_t *lengths, int B,
+                       int H, int group, int D, int W, int page_size, int n_pages, float scale,
+                       void *workspace, size_t workspace_bytes, void *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
