@@ -75,6 +75,9 @@ SIGNATURES = {
     "escha_paged_attend_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "escha_paged_attend": (_i, [_vp, ctypes.c_long, ctypes.c_long, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp,
                                 _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _vp]),
+    "escha_sample": (_i, [_vp, _i, ctypes.c_long, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp,
+                          _vp]),
+    "escha_sample_max_vocab": (_i, [_i]),
     "escha_moe_shared_finish": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

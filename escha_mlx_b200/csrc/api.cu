@@ -1088,4 +1088,35 @@ int escha_paged_attend(const void* q, long q_row, long q_head, int q_type, const
     return ESCHA_OK;
 }
 
+int escha_sample_max_vocab(int type) {
+    return type == ESCHA_F16 || type == ESCHA_BF16 || type == ESCHA_F32 ? escha::sample_max_vocab(type) : 0;
+}
+
+int escha_sample(const void* logits, int type, long stride, int B, int V, const float* uniforms,
+                 const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                 const float* top_p, float top_p1, const float* min_p, float min_p1,
+                 int64_t* tokens, void* stream) {
+    REQUIRE(type == ESCHA_F16 || type == ESCHA_BF16 || type == ESCHA_F32,
+            "%s: logits of type %d are neither binary16, bfloat16 nor binary32", __func__, type);
+    REQUIRE(B >= 1 && B <= 1 << 24, "%s: B=%d outside [1, 2^24]", __func__, B);
+    REQUIRE(V >= 1 && V <= escha::sample_max_vocab(type), "%s: V=%d outside [1, %d]", __func__, V,
+            escha::sample_max_vocab(type));
+    REQUIRE(stride >= 0, "%s: stride=%ld is negative", __func__, stride);
+    const uintptr_t size = type == ESCHA_F32 ? 4 : 2;
+    REQUIRE(logits != nullptr, "%s: logits is NULL", __func__);
+    REQUIRE(reinterpret_cast<uintptr_t>(logits) % size == 0, "%s: logits is not aligned to its type",
+            __func__);
+    REQUIRE_WORDS(uniforms);
+    REQUIRE(aligned4(temperature) && aligned4(top_k) && aligned4(top_p) && aligned4(min_p),
+            "%s: settings are not 4-byte aligned", __func__);
+    REQUIRE(tokens != nullptr && reinterpret_cast<uintptr_t>(tokens) % 8 == 0,
+            "%s: tokens is NULL or not 8-byte aligned", __func__);
+    escha::SampleParams p{};
+    p.logits = logits; p.uniforms = uniforms;
+    p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
+    p.temperature1 = temperature1; p.top_k1 = top_k1; p.top_p1 = top_p1; p.min_p1 = min_p1;
+    p.tokens = tokens; p.stride = stride; p.B = B; p.V = V;
+    return cuda_result(escha::launch_sample(p, type, as_stream(stream)), "escha_sample");
+}
+
 }  // extern "C"

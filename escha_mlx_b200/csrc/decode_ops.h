@@ -74,4 +74,21 @@ AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, in
 cudaError_t launch_attend(const AttendParams& p, int q_type, int cache_type, bool split,
                           cudaStream_t st);
 
+struct SampleParams {
+    const void* logits;      // [B, V], rows `stride` elements apart
+    const float* uniforms;   // [B]
+    // per row, or NULL for the number beside it
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    float temperature1, top_p1, min_p1;
+    int top_k1;
+    int64_t* tokens;         // [B]
+    long stride;
+    int B, V, slice;
+};
+int sample_max_vocab(int type);
+cudaError_t launch_sample(const SampleParams& p, int type, cudaStream_t st);
+
 }  // namespace escha

@@ -1,0 +1,691 @@
+// Sampling a token per row of logits from a given uniform number.
+//
+//   d_i = (x_i - max x) / T,  w_i = exp(d_i)  (0 where d_i < -30),
+//   rows ordered by (x descending, index ascending): keep the first k (top-k), then the
+//   shortest prefix that holds a share p of what is kept (top-p), then w_i >= min_p,
+//   token = first index, in index order, whose cumulative kept weight exceeds u * total.
+//
+// The token is a whole number that has to come out the same whatever the split, so weights are
+// computed in 64 bits and summed as fixed-point integers of 44 fractional bits (262144 of them
+// stay far below 2^64): sums do not depend on their order, borders move by 2^-45 per token.
+//
+// A thread-block cluster holds one row in the shared memory of its CTAs (the row is read from
+// HBM once) and agrees on maxima, counts and sums through distributed shared memory.  Nothing
+// is sorted as a whole: a histogram over 2047 bins of d (monotone in x) bounds the part of the
+// row that can be kept, from counts alone (a bin's weights differ by 1.5%, so the nucleus is
+// bounded from above).  Where at most kList tokens are left, one CTA sorts those and settles
+// everything exactly; otherwise the cut is found bin by bin, from exact weights per bin, and
+// inside its bin by sorting it or, if ties make it large, by halving the range of values.
+// Bound by latency at small batches, by the 64-bit exponentials at large ones.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdlib>
+#include <cstring>
+#include <utility>
+
+#include "common.cuh"
+#include "decode_ops.h"
+#include "kernels.h"
+
+namespace cg = cooperative_groups;
+
+namespace escha {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;                 // the last one is not counted: weight 0
+constexpr int kList = 2048;
+constexpr float kCut = -30.0f;
+constexpr int kFraction = 44;
+constexpr float kBinsPerNat = (kBins - 1) / 30.25f;
+typedef unsigned long long u64;
+
+template <typename T> __device__ __forceinline__ float to_float(T x);
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_float(float x) { return x; }
+
+// Order-preserving key of a value; NaN counts as -inf, -0 as +0.
+__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : __int_as_float(0xff800000); }
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+struct Shared {
+    double pow2[32];                        // 2^(j / 32)
+    u64 best;                               // this CTA's largest (key, ~index)
+    u64 sum;                                // this CTA's sum of weights
+    u64 warp_sum[kWarps];
+    u64 scan[kWarps];
+    uint32_t warp_ties[kWarps];
+    uint32_t scan32[kWarps];
+    float scanf[kWarps];
+    uint32_t ties;                          // this CTA's tokens at the cut
+    uint32_t count;                         // a count exchanged between CTAs
+    uint32_t found;                         // a thread's find, for its CTA
+    uint32_t found_above;
+    uint32_t list_n;                        // (leader) tokens in the list
+    uint32_t cut_key;                       // (leader) the cut, for all CTAs
+    uint32_t cut_ties;
+    u64 bin_above;
+    __align__(16) uint32_t hist[kBins];     // counts of this CTA
+    __align__(16) uint32_t cum[kBins];      // counts of the row, inclusive prefix
+    __align__(16) u64 list[kList];          // (leader) tokens as (key, ~index); or per-bin weights
+};
+
+// Weight of a token in units of 2^-44.  2^(y / 32) = 2^(n / 32) * exp(r): a table for the
+// 32nds, a Taylor series of degree 5 for |r| <= ln 2 / 64 (remainder below 3e-15).
+struct Weights {
+    double top, inv;
+    float topf;
+    const double* pow2;
+    __device__ __forceinline__ u64 operator()(float x) const {
+        if (x == topf) return 1ull << kFraction;
+        const double d = (static_cast<double>(x) - top) * inv;
+        if (!(d >= static_cast<double>(kCut))) return 0;
+        const double y = d * 46.166241308446828384;                  // 32 log2(e)
+        const double magic = 6755399441055744.0;                     // 1.5 * 2^52: rounds to integer
+        const double shifted = y + magic;
+        const int n = static_cast<int>(__double_as_longlong(shifted));
+        const double r = (y - (shifted - magic)) * 0.021660849392498290;   // ln 2 / 32
+        double e = 1.0 / 120.0;
+        e = fma(e, r, 1.0 / 24.0);
+        e = fma(e, r, 1.0 / 6.0);
+        e = fma(e, r, 0.5);
+        e = fma(e, r, 1.0);
+        e = fma(e, r, 1.0);
+        const long long scale = static_cast<long long>((n >> 5) + kFraction) << 52;
+        const double t = __longlong_as_double(__double_as_longlong(pow2[n & 31]) + scale);
+        // t * e <= 2^44: adding 2^52 leaves the nearest integer in the low mantissa bits
+        return static_cast<u64>(__double_as_longlong(fma(t, e, 4503599627370496.0))) & 0xfffffffffffffull;
+    }
+};
+
+template <typename V>
+__device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
+// Inclusive prefix of a value per thread over the CTA; `scratch` one word per warp.
+template <typename V>
+__device__ __forceinline__ V block_inclusive(V v, V* scratch, V* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const V o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    V base = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const V s = scratch[w];
+        if (w < warp) base += s;
+        all += s;
+    }
+    *total = all;
+    return v + base;
+}
+
+// Ascending bitonic sort of n (a power of two, at least 2) words by the CTA.
+__device__ void sort_words(u64* a, int n) {
+    for (int k = 2; k <= n; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+                const int lo = 2 * i - (i & (j - 1));
+                const int hi = lo + j;
+                const u64 x = a[lo], y = a[hi];
+                if ((x > y) == ((lo & k) == 0)) {
+                    a[lo] = y;
+                    a[hi] = x;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+__device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    Shared& s = *reinterpret_cast<Shared*>(smem);
+    T* xs = reinterpret_cast<T*>(smem + sizeof(Shared));
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = cluster.block_rank(), ctas = cluster.num_blocks();
+    const int row = blockIdx.x / ctas;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    grid_launch_dependents();
+    if (tid < 32) s.pow2[tid] = exp2(tid / 32.0);
+    if (tid == 0) s.list_n = 0;
+    grid_dependency_wait();
+
+    // ---- the CTA's slice, and the row's maximum with its lowest index
+    const int base = rank * p.slice;
+    const int n = min(max(p.V - base, 0), p.slice);
+    const T* src = static_cast<const T*>(p.logits) + static_cast<long>(row) * p.stride + base;
+    u64 best = 0;
+    auto take = [&](int i, T raw) {
+        xs[i] = raw;
+        const u64 k = static_cast<u64>(key_of(clean(to_float(raw)))) << 32 | (0xffffffffu - (base + i));
+        best = k > best ? k : best;
+    };
+    constexpr int kVec = 16 / sizeof(T);
+    int done = 0;
+    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        for (int i = tid * kVec; i + kVec <= n; i += kThreads * kVec) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src + i);
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) take(i + k, e[k]);
+        }
+        done = n / kVec * kVec;
+    }
+#pragma unroll 4
+    for (int i = done + tid; i < n; i += kThreads) take(i, src[i]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        const u64 o = __shfl_xor_sync(0xffffffffu, best, d);
+        best = o > best ? o : best;
+    }
+    if (lane == 0) s.scan[warp] = best;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) best = s.scan[w] > best ? s.scan[w] : best;
+        s.best = best;
+    }
+    for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
+    cluster.sync();
+    best = 0;
+    for (int r = 0; r < ctas; ++r) {
+        const u64 o = *cluster.map_shared_rank(&s.best, r);
+        best = o > best ? o : best;
+    }
+    const float top = value_of(static_cast<uint32_t>(best >> 32));
+    const int top_index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+    const float temperature = p.temperature ? p.temperature[row] : p.temperature1;
+    const bool empty = top == __int_as_float(0xff800000);
+    if (empty || !(temperature > 0.0f)) {
+        if (rank == 0 && tid == 0) p.tokens[row] = empty ? -1 : top_index;
+        cluster.sync();                     // no CTA leaves while its memory is read
+        return;
+    }
+    const int k = p.top_k ? p.top_k[row] : p.top_k1;
+    const float share = fmaxf(p.top_p ? p.top_p[row] : p.top_p1, 0.0f);
+    const float least = fminf(p.min_p ? p.min_p[row] : p.min_p1, 1.0f);
+    const float u = p.uniforms[row];
+    bool k_on = k > 0 && k < p.V;
+    const bool p_on = (p.top_p ? p.top_p[row] : p.top_p1) < 1.0f, m_on = least > 0.0f;
+    const u64 least_w = m_on ? static_cast<u64>(ceil(static_cast<double>(least) * (1ull << kFraction))) : 0;
+
+    Weights weight;
+    weight.top = top;
+    weight.topf = top;
+    weight.inv = 1.0 / static_cast<double>(temperature);
+    weight.pow2 = s.pow2;
+    const float invf = 1.0f / temperature;
+    auto value = [&](int i) { return clean(to_float(xs[i])); };
+    auto bin_of = [&](float x) {
+        if (x == top) return 0;
+        const float z = (top - x) * invf * kBinsPerNat;
+        return z < static_cast<float>(kBins - 1) ? static_cast<int>(z) : kBins - 1;
+    };
+    // token to take from a total, as a cumulative weight that has to be exceeded
+    auto target_of = [&](u64 total) {
+        const double t = floor(static_cast<double>(u) * static_cast<double>(total));
+        const u64 most = total - 1;
+        return t >= static_cast<double>(most) ? most : t > 0.0 ? static_cast<u64>(t) : 0ull;
+    };
+
+    // ---- the cut: kept are keys above cut_key and the first cut_ties (by index) at it
+    uint32_t cut_key = 0, cut_ties = 0xffffffffu;
+    if (k_on || p_on || m_on) {
+        u64 sum = 0;
+        for (int i = tid; i < n; i += kThreads) {
+            const float x = value(i);
+            const int b = bin_of(x);
+            if (b < kBins - 1) {
+                atomicAdd(&s.hist[b], 1u);
+                if (p_on && !k_on) sum += weight(x);
+            }
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) s.warp_sum[warp] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            sum = 0;
+            for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
+            s.sum = sum;
+        }
+        cluster.sync();
+        u64 all = 0;                                      // weight of the row (p_on && !k_on)
+        uint4 c = make_uint4(0, 0, 0, 0);                 // bins 4 tid .. 4 tid + 3
+        for (int r = 0; r < ctas; ++r) {
+            const uint4 o = reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.hist, r))[tid];
+            c.x += o.x; c.y += o.y; c.z += o.z; c.w += o.w;
+            all += *cluster.map_shared_rank(&s.sum, r);
+        }
+        uint32_t counted;
+        const uint32_t mine = c.x + c.y + c.z + c.w;
+        const uint32_t inc = block_inclusive(mine, s.scan32, &counted);
+        const uint32_t c0 = inc - mine + c.x, c1 = c0 + c.y, c2 = c1 + c.z;
+        reinterpret_cast<uint4*>(s.cum)[tid] = make_uint4(c0, c1, c2, inc);
+        // tokens past the counted bins weigh nothing, so a top-k that reaches them cuts nothing
+        k_on = k_on && static_cast<uint32_t>(k) <= counted;
+        if (tid == 0) s.found = kBins - 1;
+        __syncthreads();
+        int k_bin = kBins - 1;
+        if (k_on) {
+            const uint32_t kk = k;
+            if (inc - mine < kk && kk <= inc)
+                s.found = 4 * tid + (kk <= c0 ? 0 : kk <= c1 ? 1 : kk <= c2 ? 2 : 3);
+            __syncthreads();
+            k_bin = s.found;
+        }
+        int m_bin = kBins - 1;
+        if (m_on) m_bin = min(kBins - 1, static_cast<int>((-logf(least) + 1e-3f) * kBinsPerNat));
+        int p_bin = kBins - 1;
+        // the weight of the row was summed only without top-k; a top-k that turned out to cut
+        // nothing takes the exact way below
+        const bool have_all = p_on && !(k > 0 && k < p.V);
+        if (have_all) {
+            // least weight that a bin's tokens can have, less a thousandth for rounding
+            auto low = [](int b) { return exp2f((b + 1) * (-1.44269504f / kBinsPerNat)) * 0.999f; };
+            const float w0 = c.x * low(4 * tid), w1 = w0 + c.y * low(4 * tid + 1);
+            const float w2 = w1 + c.z * low(4 * tid + 2), w3 = w2 + c.w * low(4 * tid + 3);
+            float total;
+            const float before = block_inclusive(w3, s.scanf, &total) - w3;
+            const float want = share * (static_cast<float>(all) * 0x1p-44f) * 1.0001f;
+            if (tid == 0) s.found = kBins - 1;
+            __syncthreads();
+            if (before + w3 >= want) {                    // the first such bin
+                const int b = 4 * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
+                                         : before + w2 >= want ? 2 : 3);
+                atomicMin(&s.found, static_cast<uint32_t>(b));
+            }
+            __syncthreads();
+            p_bin = s.found;
+        }
+        const int bound = k_on ? (p_on ? k_bin : min(k_bin, m_bin)) : p_on && !have_all ? kBins - 1
+                                                                      : min(p_bin, m_bin);
+        const uint32_t kept = s.cum[bound];
+        Shared* leader = cluster.map_shared_rank(&s, 0);
+        // tokens of bins [from, to] to the leader's list
+        auto gather = [&](int from, int to) {
+            for (int i0 = warp * 32; i0 < n; i0 += kThreads) {
+                const int i = i0 + lane;
+                const float x = i < n ? value(i) : 0.0f;
+                const int b = i < n ? bin_of(x) : kBins;
+                const bool in = b >= from && b <= to && b < kBins - 1;
+                const unsigned m = __ballot_sync(0xffffffffu, in);
+                if (m == 0) continue;
+                uint32_t at = 0;
+                if (lane == __ffs(m) - 1) at = atomicAdd(&leader->list_n, __popc(m));
+                at = __shfl_sync(0xffffffffu, at, __ffs(m) - 1) + __popc(m & ((1u << lane) - 1));
+                // sorted ascending: largest value, then lowest index, first
+                if (in) leader->list[at] = ~(static_cast<u64>(key_of(x)) << 32 | (0xffffffffu - (base + i)));
+            }
+        };
+        if (kept <= kList) {
+            // ---- everything that can be kept fits the list: one CTA settles the row
+            gather(0, bound);
+            cluster.sync();
+            if (rank == 0) {
+                const int cnt = kept, m2 = power_of_two(cnt);
+                for (int i = cnt + tid; i < m2; i += kThreads) s.list[i] = ~0ull;
+                sort_words(s.list, m2);
+                constexpr int kEach = kList / kThreads;
+                u64 w[kEach], mine_w = 0, kept_w = 0;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int i = tid * kEach + e;
+                    w[e] = i < cnt ? weight(value_of(static_cast<uint32_t>(~s.list[i] >> 32))) : 0;
+                    if (k_on && i >= k) w[e] = 0;
+                    mine_w += w[e];
+                }
+                u64 total;
+                u64 before = block_inclusive(mine_w, s.scan, &total) - mine_w;
+                const double want = static_cast<double>(share) * static_cast<double>(have_all ? all : total);
+                uint32_t at[kEach];
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int i = tid * kEach + e;
+                    bool keep = i < cnt && w[e] != 0 && w[e] >= least_w;
+                    if (p_on) keep = keep && (i == 0 || static_cast<double>(before) < want);
+                    before += w[e];
+                    if (!keep) w[e] = 0;
+                    kept_w += w[e];
+                    at[e] = i < cnt ? static_cast<uint32_t>(~s.list[i]) : 0;     // ~index
+                }
+                block_inclusive(kept_w, s.scan, &total);
+                // cumulative weights in index order: sort by index, carrying the position
+                u64* order = s.list;
+                u64* w_at = reinterpret_cast<u64*>(s.hist);        // hist and cum: 2048 words
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int i = tid * kEach + e;
+                    if (i < m2) order[i] = i < cnt ? static_cast<u64>(0xffffffffu - at[e]) << 32 | i : ~0ull;
+                    w_at[i] = w[e];
+                }
+                sort_words(order, m2);
+                u64 o[kEach];
+                mine_w = 0;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int i = tid * kEach + e;
+                    o[e] = i < cnt ? order[i] : 0;
+                    w[e] = i < cnt ? w_at[static_cast<uint32_t>(o[e])] : 0;
+                    mine_w += w[e];
+                }
+                u64 again;
+                before = block_inclusive(mine_w, s.scan, &again) - mine_w;
+                const u64 want_u = target_of(total);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    if (before <= want_u && want_u < before + w[e]) p.tokens[row] = static_cast<int>(o[e] >> 32);
+                    before += w[e];
+                }
+            }
+            cluster.sync();
+            return;
+        }
+
+        // ---- the cut bin by bin.  Sum of a count and a weight over the cluster.
+        auto agree = [&](uint32_t cnt, u64 w, uint32_t* all_cnt, u64* all_w) {
+            cnt = warp_sum(cnt);
+            w = warp_sum(w);
+            if (lane == 0) { s.scan32[warp] = cnt; s.warp_sum[warp] = w; }
+            __syncthreads();
+            if (tid == 0) {
+                cnt = 0; w = 0;
+                for (int i = 0; i < kWarps; ++i) { cnt += s.scan32[i]; w += s.warp_sum[i]; }
+                s.count = cnt; s.sum = w;
+            }
+            cluster.sync();
+            *all_cnt = 0; *all_w = 0;
+            for (int r = 0; r < ctas; ++r) {
+                *all_cnt += *cluster.map_shared_rank(&s.count, r);
+                *all_w += *cluster.map_shared_rank(&s.sum, r);
+            }
+            cluster.sync();
+        };
+        // Inside bin `bin`: the value and its ties at which the first `count` tokens, or the
+        // shortest prefix with a weight of at least `need`, end.
+        auto cut_in_bin = [&](int bin, uint32_t size, bool by_count, uint32_t count, u64 need) {
+            if (size <= kList) {
+                gather(bin, bin);
+                cluster.sync();
+                if (rank == 0) {
+                    const int m2 = power_of_two(size);
+                    for (int i = size + tid; i < m2; i += kThreads) s.list[i] = ~0ull;
+                    sort_words(s.list, m2);
+                    constexpr int kEach = kList / kThreads;
+                    u64 w[kEach], mine_w = 0;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        const int i = tid * kEach + e;
+                        const uint32_t key = static_cast<uint32_t>(~s.list[i] >> 32);
+                        w[e] = i < size && (key > cut_key || key == cut_key) ? weight(value_of(key)) : 0;
+                        mine_w += w[e];
+                    }
+                    u64 total;
+                    u64 before = block_inclusive(mine_w, s.scan, &total) - mine_w;
+                    if (tid == 0) s.found = size - 1;
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        const int i = tid * kEach + e;
+                        // last token kept: the count-th, or the first that reaches `need`
+                        if (i < size && (by_count ? i + 1u == count : before < need && before + w[e] >= need))
+                            s.found = i;
+                        before += w[e];
+                    }
+                    __syncthreads();
+                    const int last = s.found;
+                    const uint32_t key = static_cast<uint32_t>(~s.list[last] >> 32);
+                    uint32_t ties = 0;
+                    for (int i = tid; i <= last; i += kThreads)
+                        ties += static_cast<uint32_t>(~s.list[i] >> 32) == key;
+                    ties = warp_sum(ties);
+                    if (lane == 0) s.scan32[warp] = ties;
+                    __syncthreads();
+                    if (tid == 0) {
+                        ties = 0;
+                        for (int i = 0; i < kWarps; ++i) ties += s.scan32[i];
+                        s.cut_key = key;
+                        s.cut_ties = ties;
+                        s.list_n = 0;
+                    }
+                }
+                cluster.sync();
+                cut_key = leader->cut_key;
+                cut_ties = leader->cut_ties;
+                cluster.sync();
+                return;
+            }
+            // largest key t with enough tokens (weight) at or above it, bit by bit
+            uint32_t t = 0, above = 0;
+            u64 above_w = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t trial = t | 1u << bit;
+                uint32_t cnt = 0;
+                u64 w = 0;
+                for (int i = tid; i < n; i += kThreads) {
+                    const float x = value(i);
+                    if (bin_of(x) == bin && key_of(x) >= trial && key_of(x) >= cut_key) {
+                        ++cnt;
+                        if (!by_count) w += weight(x);
+                    }
+                }
+                uint32_t all_cnt;
+                u64 all_w;
+                agree(cnt, w, &all_cnt, &all_w);
+                if (by_count ? all_cnt >= count : all_w >= need) t = trial;
+                else { above = all_cnt; above_w = all_w; }
+            }
+            // `above` counts the tokens above t: the last trial that failed was the next key up
+            uint32_t ties = count - above;
+            if (!by_count) {
+                const u64 w = weight(value_of(t));
+                ties = w ? static_cast<uint32_t>((need - above_w + w - 1) / w) : 0xffffffffu;
+            }
+            cut_ties = t == cut_key ? min(ties, cut_ties) : ties;
+            cut_key = t;
+        };
+        if (k_on) {
+            const uint32_t above = k_bin ? s.cum[k_bin - 1] : 0;
+            cut_in_bin(k_bin, s.cum[k_bin] - above, true, k - above, 0);
+        }
+        if (p_on) {
+            // exact weights per bin of what is kept so far: low and high words with a carry
+            uint32_t* lo = reinterpret_cast<uint32_t*>(s.list);
+            uint32_t* hi = lo + kBins;
+            for (int i = tid; i < kBins; i += kThreads) lo[i] = hi[i] = 0;
+            // ties at a top-k cut: only cut_ties of them count, all in one bin, of one weight
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+                const float x = value(i);
+                const uint32_t key = key_of(x);
+                if (k_on ? key <= cut_key : false) continue;
+                const int b = bin_of(x);
+                if (b >= kBins - 1) continue;
+                const u64 w = weight(x);
+                if (w == 0) continue;
+                const uint32_t wl = static_cast<uint32_t>(w);
+                const uint32_t old = atomicAdd(&lo[b], wl);
+                const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + wl < old);
+                if (up) atomicAdd(&hi[b], up);
+            }
+            cluster.sync();
+            u64 wb[4] = {0, 0, 0, 0};
+            for (int r = 0; r < ctas; ++r) {
+                const uint32_t* rl = cluster.map_shared_rank(lo, r);
+                const uint4 l = reinterpret_cast<const uint4*>(rl)[tid];
+                const uint4 h = reinterpret_cast<const uint4*>(rl + kBins)[tid];
+                wb[0] += static_cast<u64>(h.x) << 32 | 0; wb[0] += l.x;
+                wb[1] += static_cast<u64>(h.y) << 32 | 0; wb[1] += l.y;
+                wb[2] += static_cast<u64>(h.z) << 32 | 0; wb[2] += l.z;
+                wb[3] += static_cast<u64>(h.w) << 32 | 0; wb[3] += l.w;
+            }
+            u64 tie_w = 0;
+            if (k_on) {
+                tie_w = weight(value_of(cut_key));
+                const int b = bin_of(value_of(cut_key));
+                if (b >> 2 == tid && b < kBins - 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((b & 3) == e) wb[e] += tie_w * cut_ties;
+                }
+            }
+            u64 total;
+            const u64 sum4 = wb[0] + wb[1] + wb[2] + wb[3];
+            u64 before = block_inclusive(sum4, s.scan, &total) - sum4;
+            const double want_d = ceil(static_cast<double>(share) * static_cast<double>(total));
+            u64 want = want_d > 1.0 ? static_cast<u64>(want_d) : 1ull;
+            if (want > total) want = total;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (before < want && before + wb[e] >= want) {
+                    s.found = 4 * tid + e;
+                    s.bin_above = before;
+                }
+                before += wb[e];
+            }
+            __syncthreads();
+            const int bin = s.found;
+            const u64 need = want - s.bin_above;
+            cluster.sync();                               // the per-bin weights are read
+            cut_in_bin(bin, s.cum[bin] - (bin ? s.cum[bin - 1] : 0), false, 0, need);
+        }
+    }
+
+    // ---- cumulative weights in index order: contiguous pieces per warp
+    const int per = ((n + kWarps - 1) / kWarps + 31) & ~31;
+    const int lo = min(warp * per, n), hi = min(lo + per, n);
+    uint32_t tie_base = 0;
+    const bool cut = cut_ties != 0xffffffffu;
+    if (cut) {
+        uint32_t ties = 0;
+        for (int i = lo + lane; i < hi; i += 32) ties += key_of(value(i)) == cut_key;
+        ties = warp_sum(ties);
+        if (lane == 0) s.warp_ties[warp] = ties;
+        __syncthreads();
+        if (tid == 0) {
+            ties = 0;
+            for (int w = 0; w < kWarps; ++w) ties += s.warp_ties[w];
+            s.ties = ties;
+        }
+        cluster.sync();
+        for (int r = 0; r < rank; ++r) tie_base += *cluster.map_shared_rank(&s.ties, r);
+        for (int w = 0; w < warp; ++w) tie_base += s.warp_ties[w];
+    }
+    // kept weight of token i of this warp's piece; `seen` ties lie before the 32 it belongs to
+    auto kept_weight = [&](int i, uint32_t& seen) {
+        const float x = i < hi ? value(i) : 0.0f;
+        const uint32_t key = i < hi ? key_of(x) : 0;
+        bool keep = i < hi && key >= cut_key;
+        if (cut) {
+            const bool tie = i < hi && key == cut_key;
+            const unsigned m = __ballot_sync(0xffffffffu, tie);
+            if (tie) keep = seen + __popc(m & ((1u << lane) - 1)) < cut_ties;
+            seen += __popc(m);
+        }
+        u64 w = keep ? weight(x) : 0;
+        return w >= least_w ? w : 0;
+    };
+    u64 sum = 0;
+    uint32_t seen = tie_base;
+    for (int i = lo; i < hi; i += 32) sum += kept_weight(i + lane, seen);
+    sum = warp_sum(sum);
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        sum = 0;
+        for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
+        s.sum = sum;
+    }
+    cluster.sync();
+    u64 total = 0, before = 0;
+    for (int r = 0; r < ctas; ++r) {
+        const u64 o = *cluster.map_shared_rank(&s.sum, r);
+        if (r < rank) before += o;
+        total += o;
+    }
+    for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
+    const u64 want = target_of(total);
+    if (before <= want && want < before + s.warp_sum[warp]) {
+        seen = tie_base;
+        for (int i = lo; i < hi; i += 32) {
+            const u64 w = kept_weight(i + lane, seen);
+            u64 inc = w;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const u64 o = __shfl_up_sync(0xffffffffu, inc, d);
+                if (lane >= d) inc += o;
+            }
+            const u64 upto = before + inc;
+            if (upto - w <= want && want < upto) p.tokens[row] = base + i + lane;
+            before += __shfl_sync(0xffffffffu, inc, 31);
+            if (before > want) break;
+        }
+    }
+    cluster.sync();
+}
+
+template <typename T>
+cudaError_t launch(SampleParams p, int ctas, cudaStream_t st) {
+    static SmemLimit limit;
+    const size_t smem = sizeof(Shared) + (static_cast<size_t>(p.slice) * sizeof(T) + 15) / 16 * 16;
+    cudaError_t e = limit.ensure(sample_kernel<T>, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.B) * ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_allowed() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+}
+
+}  // namespace
+
+int sample_max_vocab(int type) {
+    const int bytes = 227 * 1024 - static_cast<int>(sizeof(Shared)) - 16;
+    return 8 * (bytes / (type == kF32 ? 4 : 2) / 8 * 8);
+}
+
+cudaError_t launch_sample(const SampleParams& p0, int type, cudaStream_t st) {
+    SampleParams p = p0;
+    const int size = type == kF32 ? 4 : 2;
+    // CTAs per row: eight share a long row's latency; a slice below a few thousand tokens is
+    // not worth another CTA
+    int ctas = 1;
+    while (ctas < 8 && (p.V + ctas - 1) / ctas > 4096) ctas *= 2;
+    p.slice = ((p.V + ctas - 1) / ctas + 16 / size - 1) / (16 / size) * (16 / size);
+    if (type == kF16) return launch<__half>(p, ctas, st);
+    if (type == kBF16) return launch<__nv_bfloat16>(p, ctas, st);
+    return launch<float>(p, ctas, st);
+}
+
+}  // namespace escha

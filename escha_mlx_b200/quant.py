@@ -172,6 +172,13 @@ def q8_head(x: torch.Tensor, w8: torch.Tensor, scale: torch.Tensor,
 class EschaQ8Head(EschaQ8Linear):
     """int8 vocabulary head (reference :243-257); every row count takes the same kernel."""
 
+    def sample(self, x: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+               min_p=0.0) -> torch.Tensor:
+        """A token per row of ``x`` [..., K]: ``sampling.sample`` of the head's logits.  (mlx-lm's
+        part in the reference.)"""
+        from . import sampling
+        return sampling.sample(self.forward(x), uniforms, temperature, top_k, top_p, min_p)
+
 
 class EschaQ8Embedding(torch.nn.Module):
     """Embedding over an int8 table with per-row scale (reference :260-273):

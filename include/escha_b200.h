@@ -496,6 +496,24 @@ int escha_paged_attend(const void *q, long q_row, long q_head, int q_type, const
                        int H, int group, int D, int W, int page_size, int n_pages, float scale,
                        void *workspace, size_t workspace_bytes, void *out, void *stream);
 
+/* One token per row of logits [B, V] (rows `stride` elements apart; ESCHA_F16, ESCHA_BF16 or
+ * ESCHA_F32) from uniforms [B] in [0, 1).  With d_i = (x_i - max x) / temperature and weights
+ * exp(d_i), 0 where d_i < -30: of the tokens ordered by (x descending, index ascending) keep
+ * the first top_k, of those the shortest prefix with at least top_p of their weight, of those
+ * the ones with at least min_p of the largest weight; the token is the first, in index order,
+ * whose cumulative kept weight exceeds uniform * total.  temperature not above 0: the first
+ * largest; top_k outside [1, V), top_p not below 1 and min_p not above 0 cut nothing.  NaN
+ * logits count as -inf; a row without a logit above -inf gives -1.  Each setting is an array
+ * [B], or NULL for the one number after it.  Weights and sums are 64-bit: the token does not
+ * depend on how a row is split. */
+int escha_sample(const void *logits, int type, long stride, int B, int V, const float *uniforms,
+                 const float *temperature, float temperature1, const int32_t *top_k, int top_k1,
+                 const float *top_p, float top_p1, const float *min_p, float min_p1,
+                 int64_t *tokens, void *stream);
+
+/* The longest row escha_sample takes for logits of that type. */
+int escha_sample_max_vocab(int type);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,3 +99,29 @@ def test_python_level_refusals_without_a_gpu():
     i = torch.zeros((1, 1), dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
         paged.plan_pages(i, i[0], i[0], i[0], i[0], page_size=16, n_pages=4, rows=1)
+
+
+def sample(logits=P, kind=0, stride=8, B=1, V=8, u=P, tokens=P):
+    return lib.escha_sample(logits, kind, stride, B, V, u, None, 1.0, None, 0, None, 1.0, None, 0.0,
+                            tokens, None)
+
+
+def test_sample_refusals():
+    refused(sample(kind=3), "type 3")
+    refused(sample(B=0), "B=0")
+    refused(sample(V=0), "V=0")
+    refused(sample(V=lib.escha_sample_max_vocab(0) + 1), "V=")
+    refused(sample(kind=2, V=lib.escha_sample_max_vocab(0)), "V=")
+    refused(sample(stride=-1), "stride=-1")
+    refused(sample(logits=None), "logits is NULL")
+    refused(sample(logits=ctypes.c_void_p(0x1001)), "aligned")
+    refused(sample(u=None), "uniforms is NULL")
+    refused(sample(tokens=None), "tokens is NULL")
+    refused(sample(tokens=ctypes.c_void_p(0x1004)), "8-byte")
+    assert lib.escha_sample_max_vocab(0) >= 2 * lib.escha_sample_max_vocab(2) - 64 >= 300000
+    assert lib.escha_sample_max_vocab(7) == 0
+    from escha_mlx_b200 import sampling
+    with pytest.raises(ValueError, match="CUDA"):
+        sampling.sample(torch.zeros((1, 8)), torch.zeros(1))
+    with pytest.raises(ValueError, match="logits"):
+        sampling.max_vocab(torch.float64)
