@@ -15,7 +15,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import moe, quant
+from . import moe, paged, quant
 from .models.qwen3_5_moe import EschaSparseMoeBlock
 
 MOE_35B = dict(hidden=2048, inter=512, experts=256, top_k=8, K_gate_up=2, K_down=2,
@@ -46,9 +46,9 @@ def _q8(n, kd, device, gen) -> quant.EschaQ8Linear:
 class MoeLayer(torch.nn.Module):
     """One decode layer's projections on this path: [int8 q/k/v/o] + the MoE block.
 
-    Attention itself (scores, cache) is not part of the coded-projection path; the
-    o projection consumes the q projection's output so that the four int8 linears
-    run with their real shapes and dependencies.
+    ``forward`` leaves attention itself out: the o projection consumes the q projection's
+    output so that the four int8 linears run with their real shapes and dependencies.
+    ``decode`` is the same layer with its attention, over a paged cache.
     """
 
     def __init__(self, device, gen, cfg=MOE_35B, attention: bool = False,
@@ -80,6 +80,7 @@ class MoeLayer(torch.nn.Module):
             self.q, self.k, self.v = _q8(qd, H, device, gen), _q8(kvd, H, device, gen), \
                 _q8(kvd, H, device, gen)
             self.o = _q8(H, qd, device, gen)
+            self._kv_heads, self._head_dim = cfg["kv_heads"], cfg["head_dim"]
         self.expert_bytes = (H * 2 * I * cfg["K_gate_up"] + I * H * cfg["K_down"]) // 8
         self.int8_bytes = 3 * H * I + (2 * H * (qd + kvd) if attention else 0)
         self.router_bytes = 2 * E * H
@@ -92,6 +93,28 @@ class MoeLayer(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.block(self._attention_projections(x))
+
+    def new_cache(self, n_pages: int, page_size: int, dtype=torch.float16) -> paged.PagedCache:
+        """An empty paged cache of this layer's key/value heads."""
+        return paged.PagedCache(n_pages, page_size, self._kv_heads, self._head_dim, dtype,
+                                self.k._w8.device)
+
+    def attend(self, x: torch.Tensor, cache: paged.PagedCache, table: torch.Tensor,
+               plan: paged.PagePlan) -> torch.Tensor:
+        """Attention of one new token per request: int8 q/k/v projections of ``x`` [B, hidden]
+        in one launch, the new keys and values stored in ``cache``, attention over it.  Returns
+        the heads side by side, [B, q_heads * head_dim]."""
+        q, k, v = quant.project_many_q8([self.q, self.k, self.v], x)
+        heads = (lambda y: y.unflatten(1, (-1, self._head_dim)))
+        cache.append(heads(k), heads(v), plan.slots)
+        return cache.attend(heads(q), table, plan.ends).flatten(1)
+
+    def decode(self, x: torch.Tensor, cache: paged.PagedCache, table: torch.Tensor,
+               plan: paged.PagePlan) -> torch.Tensor:
+        """The layer with its attention, for one new token per request (``plan``: the step's
+        ``paged.plan_pages`` with ``rows`` = B); otherwise as ``forward``."""
+        y = self.o(self.attend(x, cache, table, plan))
+        return self.block(torch.add(x, y, alpha=0.01))
 
     def routed_experts(self, x: torch.Tensor) -> int:
         """Distinct experts of this rank's shard that the rows of ``x`` are routed to
