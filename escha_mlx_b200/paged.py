@@ -12,6 +12,7 @@ graph (``graphs.GraphedCall``) and replayed while lengths and tables change.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -26,24 +27,25 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 PLAN_MAX_BATCH = 4096
 
 
-class on_device:
-    """Runs the enclosed calls on a tensor's device, whichever device is current, and gives
-    that device's current stream."""
+_raw_stream = torch._C._cuda_getCurrentRawStream     # (device index) -> current stream's handle
+_current_device = torch.cuda.current_device
 
-    __slots__ = ("_want", "_was")
 
-    def __init__(self, device: torch.device) -> None:
-        self._want = device.index
+def call_on(index: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of device ``index``, whichever device is
+    current."""
+    if _current_device() == index:
+        check(fn(*args, _raw_stream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, _raw_stream(index)))
 
-    def __enter__(self) -> int:
-        self._was = torch.cuda.current_device()
-        if self._want is not None and self._want != self._was:
-            torch.cuda.set_device(self._want)
-        return torch.cuda.current_stream().cuda_stream
 
-    def __exit__(self, *exc) -> None:
-        if self._want is not None and self._want != self._was:
-            torch.cuda.set_device(self._was)
+def _is_int32(t, index: int, shape: tuple) -> bool:
+    """A dense int32 tensor of that shape on device ``index`` (the checks of every call, in
+    short; ``_check`` says what is wrong with one that fails)."""
+    return (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == shape
+            and t.get_device() == index and t.is_contiguous())
 
 
 def _check(name: str, t: torch.Tensor, shape: tuple, dtype, device: torch.device | None) -> None:
@@ -59,6 +61,13 @@ def _check(name: str, t: torch.Tensor, shape: tuple, dtype, device: torch.device
         raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+@functools.lru_cache(maxsize=4096)
+def _attend_workspace(index: int, *shape: int) -> int:
+    """Bytes of scratch for an attention call of that shape on that device."""
+    with torch.cuda.device(index):
+        return lib.escha_paged_attend_workspace_bytes(*shape)
 
 
 class PagePlan(NamedTuple):
@@ -83,43 +92,50 @@ def plan_pages(table: torch.Tensor, lengths: torch.Tensor, added: torch.Tensor,
     (negative numbers, more tokens than W pages hold, rows past ``rows``, free pages used up by
     it and those before it) gets nothing: its rows have slot -1, ``ends`` keeps its length and
     ``refused`` counts it.  One launch, for up to 4096 requests."""
-    _check("table", table, (None, None), torch.int32, None)
-    dev, (b, w) = table.device, table.shape
-    _check("lengths", lengths, (b,), torch.int32, dev)
-    _check("added", added, (b,), torch.int32, dev)
-    _check("free_pages", free_pages, (None,), torch.int32, dev)
-    _check("head", head, (1,), torch.int32, dev)
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        _check("table", table, (None, None), torch.int32, None)
+    (b, w), index = table.shape, table.get_device()
+    if not (index >= 0 and _is_int32(table, index, (b, w)) and _is_int32(lengths, index, (b,))
+            and _is_int32(added, index, (b,)) and _is_int32(head, index, (1,))
+            and _is_int32(free_pages, index, free_pages.shape[:1])):
+        _check("table", table, (None, None), torch.int32, None)
+        _check("lengths", lengths, (b,), torch.int32, table.device)
+        _check("added", added, (b,), torch.int32, table.device)
+        _check("free_pages", free_pages, (None,), torch.int32, table.device)
+        _check("head", head, (1,), torch.int32, table.device)
     rows = int(rows)
     if not 1 <= b <= PLAN_MAX_BATCH:
         raise ValueError(f"plan_pages takes 1..{PLAN_MAX_BATCH} requests, got {b}")
     if not 0 <= rows <= 1 << 30:
         raise ValueError(f"rows must be in [0, 2^30], got {rows}")
-    with on_device(dev) as st:
-        buf = torch.empty(2 * rows + 2 * b + 3, dtype=torch.int32, device=dev)
-        plan = PagePlan(*buf.split([rows, rows, b + 1, b, 1, 1]))
-        at = buf.data_ptr()
-        check(lib.escha_page_plan(
-            table.data_ptr(), lengths.data_ptr(), added.data_ptr(), free_pages.data_ptr(),
-            free_pages.shape[0], head.data_ptr(), b, w, page_size, n_pages, rows, at, at + 4 * rows,
-            at + 8 * rows, at + 4 * (2 * rows + b + 1), at + 4 * (2 * rows + 2 * b + 1),
-            at + 4 * (2 * rows + 2 * b + 2), st))
-    return plan
+    if page_size not in PAGE_SIZES or not 1 <= n_pages < 1 << 31:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES} and n_pages in [1, 2^31), got "
+                         f"{page_size} and {n_pages}")
+    buf = table.new_empty(2 * rows + 2 * b + 3)
+    at = buf.data_ptr()
+    ends = at + 4 * (2 * rows + b + 1)
+    call_on(index, lib.escha_page_plan, table.data_ptr(), lengths.data_ptr(), added.data_ptr(),
+            free_pages.data_ptr(), free_pages.shape[0], head.data_ptr(), b, w, page_size, n_pages, rows,
+            at, at + 4 * rows, at + 8 * rows, ends, ends + 4 * b, ends + 4 * b + 4)
+    return PagePlan(*buf.split_with_sizes((rows, rows, b + 1, b, 1, 1)))
 
 
-def _rows(name: str, x: torch.Tensor, shape: tuple, dev: torch.device) -> torch.Tensor:
-    """``x`` itself if the kernels can read it as it is (dense channels, other strides multiples
-    of 8 elements, 16-byte aligned), else a dense copy."""
+def _rows(name: str, x: torch.Tensor, shape: tuple, index: int) -> tuple:
+    """``x`` [rows, heads, channels] as the kernels can read it (dense channels, other strides
+    multiples of 8 elements, 16-byte aligned; a dense copy if it is not so), with its row and
+    head strides."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path in this package)")
-    if x.device != dev:
-        raise ValueError(f"{name} is on {x.device}, the cache on {dev}")
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, the cache on cuda:{index}")
     if x.dim() != 3 or any(w is not None and w != n for w, n in zip(shape, x.shape)):
         want = ", ".join("*" if w is None else str(w) for w in shape)
         raise ValueError(f"{name} must have shape [{want}], got {list(x.shape)}")
     s0, s1, s2 = x.stride()
-    if s2 == 1 and not (s0 | s1) & 7 and not x.data_ptr() & 15:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    if s2 != 1 or (s0 | s1) & 7 or x.data_ptr() & 15:
+        x = x.clone(memory_format=torch.contiguous_format)
+        s0, s1, s2 = x.stride()
+    return x, s0, s1
 
 
 class PagedCache:
@@ -168,12 +184,13 @@ class PagedCache:
             _check("v_scale", v_scale, tuple(k.shape[:3]), torch.float32, k.device)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.dtype, self.device = k.dtype, k.device
+        self._index = k.get_device()
+        # what every call passes on
+        self._tensors = (k.data_ptr(), v.data_ptr(), _TYPES[k.dtype],
+                         *((None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())))
 
     def arrays(self) -> list[torch.Tensor]:
         return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
-
-    def _scales(self) -> tuple:
-        return (None, None) if self.k_scale is None else (self.k_scale.data_ptr(), self.v_scale.data_ptr())
 
     def _row_type(self, name: str, x: torch.Tensor) -> int:
         ok = (torch.float16, torch.bfloat16) if self.dtype == torch.int8 else (self.dtype,)
@@ -187,20 +204,20 @@ class PagedCache:
         negative slot (or one past the cache) are skipped; the slots of one call must differ.
         Rows may be views into a merged projection (any row and head stride).  In an int8 cache
         a row becomes ``scale = max|x| / 127`` and its nearest codes, per head."""
-        k = _rows("k", k, (None, self.kv_heads, self.head_dim), self.device)
-        v = _rows("v", v, tuple(k.shape), self.device)
-        if k.dtype != v.dtype:
+        k, k_row, k_head = _rows("k", k, (None, self.kv_heads, self.head_dim), self._index)
+        t = k.shape[0]
+        v, v_row, v_head = _rows("v", v, (t, self.kv_heads, self.head_dim), self._index)
+        if k.dtype is not v.dtype:
             raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
         kind = self._row_type("k", k)
-        t = k.shape[0]
-        _check("slots", slots, (t,), torch.int32, self.device)
+        if not _is_int32(slots, self._index, (t,)):
+            _check("slots", slots, (t,), torch.int32, self.device)
         if t == 0:
             return
-        with on_device(self.device) as st:
-            check(lib.escha_paged_append(
-                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), kind,
-                slots.data_ptr(), t, self.kv_heads, self.head_dim, self.page_size, self.n_pages,
-                self.k.data_ptr(), self.v.data_ptr(), _TYPES[self.dtype], *self._scales(), st))
+        k_cache, v_cache, cache_type, k_scale, v_scale = self._tensors
+        call_on(self._index, lib.escha_paged_append, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+                v_head, kind, slots.data_ptr(), t, self.kv_heads, self.head_dim, self.page_size,
+                self.n_pages, k_cache, v_cache, cache_type, k_scale, v_scale)
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
                scale: float | None = None) -> torch.Tensor:
@@ -209,26 +226,26 @@ class PagedCache:
         ``i // (heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns
         [B, heads, head_dim] in q's type.  A request of length 0 gives zeros; tokens on pages
         outside the cache are left out; lengths past the table are cut to it."""
-        q = _rows("q", q, (None, None, self.head_dim), self.device)
+        q, q_row, q_head = _rows("q", q, (None, None, self.head_dim), self._index)
         kind = self._row_type("q", q)
         b, heads, d = q.shape
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads do not share {self.kv_heads} key/value heads evenly")
-        _check("table", table, (b, None), torch.int32, self.device)
-        _check("lengths", lengths, (b,), torch.int32, self.device)
-        group, w = heads // self.kv_heads, table.shape[1]
+        if not isinstance(table, torch.Tensor) or table.dim() != 2:
+            _check("table", table, (b, None), torch.int32, self.device)
+        group, w, index = heads // self.kv_heads, table.shape[1], self._index
+        if not (_is_int32(table, index, (b, w)) and _is_int32(lengths, index, (b,))):
+            _check("table", table, (b, None), torch.int32, self.device)
+            _check("lengths", lengths, (b,), torch.int32, self.device)
         if w < 1:
             raise ValueError("table needs at least one page per request")
-        with on_device(self.device) as st:
-            out = torch.empty((b, heads, d), dtype=q.dtype, device=self.device)
-            if b == 0:
-                return out
-            need = lib.escha_paged_attend_workspace_bytes(b, self.kv_heads, group, d, w, self.page_size)
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            check(lib.escha_paged_attend(
-                q.data_ptr(), q.stride(0), q.stride(1), kind, self.k.data_ptr(), self.v.data_ptr(),
-                _TYPES[self.dtype], *self._scales(), table.data_ptr(), lengths.data_ptr(), b,
-                self.kv_heads, group, d, w, self.page_size, self.n_pages,
-                d ** -0.5 if scale is None else float(scale), work.data_ptr() if need else None, need,
-                out.data_ptr(), st))
+        out = q.new_empty((b, heads, d))
+        if b == 0:
+            return out
+        need = _attend_workspace(index, b, self.kv_heads, group, d, w, self.page_size)
+        work = q.new_empty(need, dtype=torch.uint8) if need else None
+        call_on(index, lib.escha_paged_attend, q.data_ptr(), q_row, q_head, kind, *self._tensors,
+                table.data_ptr(), lengths.data_ptr(), b, self.kv_heads, group, d, w, self.page_size,
+                self.n_pages, d ** -0.5 if scale is None else scale, work.data_ptr() if need else None,
+                need, out.data_ptr())
         return out

@@ -8,8 +8,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import check, lib
-from .paged import on_device
+from ._lib import lib
+from .paged import call_on
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -21,15 +21,16 @@ def max_vocab(dtype: torch.dtype) -> int:
     return lib.escha_sample_max_vocab(_TYPES[dtype])
 
 
-def _setting(name: str, value, rows: int, dtype, device) -> tuple:
+def _setting(name: str, value, rows: int, dtype, index: int) -> tuple:
     """(pointer or None, number) of a setting: one number, or a tensor with one per row."""
     if not isinstance(value, torch.Tensor):
-        return None, (int(value) if dtype == torch.int32 else float(value))
-    if value.dtype != dtype or value.numel() != rows or not value.is_contiguous():
+        # any top_k past the vocabulary says the same
+        return None, (max(-1, min(int(value), 0x7fffffff)) if dtype is torch.int32 else float(value))
+    if value.dtype is not dtype or value.numel() != rows or not value.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {rows} values, "
                          f"got {value.dtype} {list(value.shape)}")
-    if value.device != device:
-        raise ValueError(f"{name} is on {value.device}, the logits on {device}")
+    if value.get_device() != index:
+        raise ValueError(f"{name} is on {value.device}, the logits on cuda:{index}")
     return value.data_ptr(), 0
 
 
@@ -51,24 +52,24 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=
         raise ValueError(f"logits must be one of {list(_TYPES)}, got {logits.dtype}")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must have shape [..., V], got {list(logits.shape)}")
-    lead, v, dev = logits.shape[:-1], logits.shape[-1], logits.device
-    x = logits if logits.dim() == 2 else logits.reshape(-1, v)
+    lead, v, index = logits.shape[:-1], logits.shape[-1], logits.get_device()
+    x = logits if len(lead) == 1 else logits.reshape(-1, v)
+    if v > 0x7fffffff:
+        raise ValueError(f"V={v} logits per row; sample takes {max_vocab(x.dtype)} at most")
     if x.stride(1) != 1:
         x = x.contiguous()
     b = x.shape[0]
-    if not isinstance(uniforms, torch.Tensor) or uniforms.dtype != torch.float32 \
+    if not isinstance(uniforms, torch.Tensor) or uniforms.dtype is not torch.float32 \
             or uniforms.shape != lead or not uniforms.is_contiguous():
         raise ValueError(f"uniforms must be a contiguous float32 tensor of shape {list(lead)}")
-    if uniforms.device != dev:
-        raise ValueError(f"uniforms is on {uniforms.device}, the logits on {dev}")
-    t, t1 = _setting("temperature", temperature, b, torch.float32, dev)
-    k, k1 = _setting("top_k", top_k, b, torch.int32, dev)
-    p, p1 = _setting("top_p", top_p, b, torch.float32, dev)
-    m, m1 = _setting("min_p", min_p, b, torch.float32, dev)
-    with on_device(dev) as st:
-        tokens = torch.empty(lead, dtype=torch.int64, device=dev)
-        if b:
-            check(lib.escha_sample(x.data_ptr(), _TYPES[x.dtype], x.stride(0), b, v,
-                                   uniforms.data_ptr(), t, t1, k, k1, p, p1, m, m1,
-                                   tokens.data_ptr(), st))
+    if uniforms.get_device() != index:
+        raise ValueError(f"uniforms is on {uniforms.device}, the logits on {logits.device}")
+    t, t1 = _setting("temperature", temperature, b, torch.float32, index)
+    k, k1 = _setting("top_k", top_k, b, torch.int32, index)
+    p, p1 = _setting("top_p", top_p, b, torch.float32, index)
+    m, m1 = _setting("min_p", min_p, b, torch.float32, index)
+    tokens = uniforms.new_empty(lead, dtype=torch.int64)
+    if b:
+        call_on(index, lib.escha_sample, x.data_ptr(), _TYPES[x.dtype], x.stride(0), b, v,
+                uniforms.data_ptr(), t, t1, k, k1, p, p1, m, m1, tokens.data_ptr())
     return tokens
