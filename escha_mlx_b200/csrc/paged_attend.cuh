@@ -136,7 +136,7 @@ struct Shape {
     static constexpr int kPiece = kRow / kSets / 16;      // bytes of a piece: 16, 8 or 4
     static constexpr int kPerPiece = kPiece / kElem;      // channels of a piece
     static constexpr int kMma = kSets * kPerPiece;        // O^T tiles of 16 channels
-    static constexpr int kScales = I8 ? 4 * 32 * 4 : 0;   // bytes of a tile's scales in the ring
+    static constexpr int kScales = I8 ? 2 * kTile * 4 : 0;   // bytes of a tile's scales in the ring
     static constexpr int kQWords = I8 ? 8 : 4;            // query words per lane and chunk
     static constexpr int kQBytes = NT * kChunks * kQWords * 4 * 32;
     static constexpr int kRingStage = kHalf + kScales;
@@ -290,12 +290,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
                     }
                     fetch_rows(dst, k_src);
                     if constexpr (I8) {
-                        const bool in0 = g < k_have, in1 = g + 8 < k_have;
-                        const uint32_t sd = dst + S::kHalf + lane * 16;
-                        copy_async<4>(sd, ks_src + (in0 ? g : 0), in0 ? 4 : 0);
-                        copy_async<4>(sd + 4, ks_src + (in1 ? g + 8 : 0), in1 ? 4 : 0);
-                        copy_async<4>(sd + 8, vs_src + (in0 ? g : 0), in0 ? 4 : 0);
-                        copy_async<4>(sd + 12, vs_src + (in1 ? g + 8 : 0), in1 ? 4 : 0);
+                        // scales: lanes 0..15 K's, the others V's
+                        const float* src = lane < kTile ? ks_src : vs_src;
+                        const bool in = (lane & 15) < k_have;
+                        copy_async<4>(dst + S::kHalf + lane * 4, src + (in ? lane & 15 : 0), in ? 4 : 0);
                     }
                 } else {
                     fetch_rows(dst, v_src);
@@ -410,7 +408,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
                 }
             }
             float4 sc = make_float4(1.0f, 1.0f, 1.0f, 1.0f);   // K's, then V's scales of tokens g, g + 8
-            if constexpr (I8) sc = reinterpret_cast<const float4*>(tile + S::kHalf)[lane];
+            if constexpr (I8) {
+                const float* scales = reinterpret_cast<const float*>(tile + S::kHalf);
+                sc = make_float4(scales[g], scales[g + 8], scales[kTile + g], scales[kTile + g + 8]);
+            }
             fetch(2 * j + S::kStages - 1, wr);
             rd = rd + 1 == S::kStages ? 0 : rd + 1;
             wr = wr + 1 == S::kStages ? 0 : wr + 1;
