@@ -38,6 +38,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;                 // the last one is not counted: weight 0
 constexpr int kList = 2048;
+constexpr int kSparse = 4096;               // listed tokens of a slice (16-bit places over the counts)
 constexpr float kCut = -30.0f;
 constexpr int kFraction = 44;
 constexpr float kBinsPerNat = (kBins - 1) / 30.25f;
@@ -47,11 +48,15 @@ template <typename T> __device__ __forceinline__ float to_float(T x);
 template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ float to_float(float x) { return x; }
+template <typename T> __device__ __forceinline__ T lowest();      // -inf
+template <> __device__ __forceinline__ __half lowest() { return __ushort_as_half(0xfc00); }
+template <> __device__ __forceinline__ __nv_bfloat16 lowest() { return __ushort_as_bfloat16(0xff80); }
+template <> __device__ __forceinline__ float lowest() { return __int_as_float(0xff800000); }
 
-// Order-preserving key of a value; NaN counts as -inf, -0 as +0.
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : __int_as_float(0xff800000); }
+// Order-preserving key of a value, the same for both zeros.  (A NaN's key is of no
+// consequence: it has no bin and no weight.)
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
@@ -64,7 +69,6 @@ struct Shared {
     u64 sum;                                // this CTA's sum of weights
     u64 warp_sum[kWarps];
     u64 scan[kWarps];
-    uint32_t warp_ties[kWarps];
     uint32_t scan32[kWarps];
     float scanf[kWarps];
     uint32_t ties;                          // this CTA's tokens at the cut
@@ -138,8 +142,31 @@ __device__ __forceinline__ V block_inclusive(V v, V* scratch, V* total) {
     return v + base;
 }
 
-// Ascending bitonic sort of n (a power of two, at least 2) words by the CTA.
-__device__ void sort_words(u64* a, int n) {
+// Sorts n distinct words ascending by the CTA (the rest up to a power of two is ~0): each to
+// the place that the number of smaller ones gives, up to kCounted of them (measured at 60:
+// 0.5 us against 2), a bitonic sort above.
+constexpr int kCounted = 256;
+__device__ void sort_words(u64* a, int count, int n, uint32_t* scratch) {
+    if (n <= kCounted) {
+        // kThreads / n threads per word, each compares with its share of the words
+        const int per = kThreads / n, i = threadIdx.x / per, part = threadIdx.x % per;
+        __syncthreads();
+        const u64 x = a[i];
+        int below = 0;
+        if (i < count)
+            for (int k = part; k < count; k += per) below += a[k] < x;
+        for (int d = 1; d < per && d < 32; d <<= 1) below += __shfl_xor_sync(0xffffffffu, below, d);
+        if (per > 32) {
+            if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = below;
+            __syncthreads();
+            below = 0;
+            for (int w = 0; w < per / 32; ++w) below += scratch[i * (per / 32) + w];
+        }
+        __syncthreads();
+        if (part == 0 && i < count) a[below] = x;
+        __syncthreads();
+        return;
+    }
     for (int k = 2; k <= n; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
             __syncthreads();
@@ -172,29 +199,52 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     if (tid == 0) s.list_n = 0;
     grid_dependency_wait();
 
-    // ---- the CTA's slice, and the row's maximum with its lowest index
+    // ---- the CTA's slice (filled up with -inf), and the row's maximum with its lowest index
     const int base = rank * p.slice;
     const int n = min(max(p.V - base, 0), p.slice);
     const T* src = static_cast<const T*>(p.logits) + static_cast<long>(row) * p.stride + base;
-    u64 best = 0;
-    auto take = [&](int i, T raw) {
-        xs[i] = raw;
-        const u64 k = static_cast<u64>(key_of(clean(to_float(raw)))) << 32 | (0xffffffffu - (base + i));
-        best = k > best ? k : best;
-    };
     constexpr int kVec = 16 / sizeof(T);
-    int done = 0;
-    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        for (int i = tid * kVec; i + kVec <= n; i += kThreads * kVec) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + i);
-            const T* e = reinterpret_cast<const T*>(&v);
+    const int vecs = p.slice / kVec;
+    uint4* const xv = reinterpret_cast<uint4*>(xs);
+    float most = __int_as_float(0xff800000);
+    int most_at = 0;
+    auto take = [&](int i, T raw) {
+        // a thread's indices ascend, so the first of equals stays
+        const float x = to_float(raw);
+        if (x > most) { most = x; most_at = i; }
+    };
+    const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    const int whole = aligned ? n / kVec : 0;             // vectors read as such
+    constexpr int kBatch = 4;                             // loads in flight per thread
+    for (int v0 = tid; v0 < whole; v0 += kBatch * kThreads) {
+        uint4 q[kBatch];
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) take(i + k, e[k]);
+        for (int j = 0; j < kBatch; ++j)
+            if (v0 + j * kThreads < whole) q[j] = reinterpret_cast<const uint4*>(src)[v0 + j * kThreads];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int v = v0 + j * kThreads;
+            if (v >= whole) break;
+            xv[v] = q[j];
+            const T* e = reinterpret_cast<const T*>(&q[j]);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) take(v * kVec + k, e[k]);
         }
-        done = n / kVec * kVec;
     }
-#pragma unroll 4
-    for (int i = done + tid; i < n; i += kThreads) take(i, src[i]);
+    for (int i0 = whole * kVec + tid; i0 < p.slice; i0 += 2 * kBatch * kThreads) {
+        T q[2 * kBatch];
+#pragma unroll
+        for (int j = 0; j < 2 * kBatch; ++j)
+            q[j] = i0 + j * kThreads < n ? src[i0 + j * kThreads] : lowest<T>();
+#pragma unroll
+        for (int j = 0; j < 2 * kBatch; ++j) {
+            const int i = i0 + j * kThreads;
+            if (i >= p.slice) break;
+            xs[i] = q[j];
+            take(i, q[j]);
+        }
+    }
+    u64 best = static_cast<u64>(key_of(most)) << 32 | (0xffffffffu - (base + most_at));
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
         const u64 o = __shfl_xor_sync(0xffffffffu, best, d);
@@ -237,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     weight.inv = 1.0 / static_cast<double>(temperature);
     weight.pow2 = s.pow2;
     const float invf = 1.0f / temperature;
-    auto value = [&](int i) { return clean(to_float(xs[i])); };
+    auto value = [&](int i) { return to_float(xs[i]); };
     auto bin_of = [&](float x) {
         if (x == top) return 0;
         const float z = (top - x) * invf * kBinsPerNat;
@@ -250,17 +300,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         return t >= static_cast<double>(most) ? most : t > 0.0 ? static_cast<u64>(t) : 0ull;
     };
 
+    // A thread's part of the slice in index order: an odd number of vectors, so that the 16-byte
+    // reads of eight neighbours fall on different banks.
+    const int part_vecs = ((vecs + kThreads - 1) / kThreads) | 1;
+    const int first_vec = min(tid * part_vecs, vecs), last_vec = min(first_vec + part_vecs, vecs);
+    // tokens of the slice that can be kept, by index (over the counts); -1: not listed
+    uint16_t* const left = reinterpret_cast<uint16_t*>(s.hist);
+    int sparse = -1;
+
     // ---- the cut: kept are keys above cut_key and the first cut_ties (by index) at it
     uint32_t cut_key = 0, cut_ties = 0xffffffffu;
     if (k_on || p_on || m_on) {
         u64 sum = 0;
-        for (int i = tid; i < n; i += kThreads) {
-            const float x = value(i);
-            const int b = bin_of(x);
-            if (b < kBins - 1) {
-                atomicAdd(&s.hist[b], 1u);
-                if (p_on && !k_on) sum += weight(x);
+        for (int v = tid; v < vecs; v += kThreads) {
+            const uint4 q = xv[v];
+            const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+                const int b = bin_of(to_float(e[k]));
+                if (b < kBins - 1) atomicAdd(&s.hist[b], 1u);
             }
+            if (p_on && !k_on)
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) sum += weight(to_float(e[k]));
         }
         sum = warp_sum(sum);
         if (lane == 0) s.warp_sum[warp] = sum;
@@ -325,18 +387,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         Shared* leader = cluster.map_shared_rank(&s, 0);
         // tokens of bins [from, to] to the leader's list
         auto gather = [&](int from, int to) {
-            for (int i0 = warp * 32; i0 < n; i0 += kThreads) {
-                const int i = i0 + lane;
-                const float x = i < n ? value(i) : 0.0f;
-                const int b = i < n ? bin_of(x) : kBins;
-                const bool in = b >= from && b <= to && b < kBins - 1;
-                const unsigned m = __ballot_sync(0xffffffffu, in);
-                if (m == 0) continue;
+            // 32 tokens per thread and round: their hits as a mask, one reservation per warp
+            constexpr int kRound = 32 / kVec;
+            for (int v0 = 0; v0 < vecs; v0 += kRound * kThreads) {
+                unsigned hits = 0;
+#pragma unroll
+                for (int j = 0; j < kRound; ++j) {
+                    const int v = v0 + j * kThreads + tid;
+                    const uint4 q = v < vecs ? xv[v] : make_uint4(0, 0, 0, 0);
+                    const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                    for (int k = 0; k < kVec; ++k) {
+                        const int b = bin_of(to_float(e[k]));
+                        if (v < vecs && b >= from && b <= to && b < kBins - 1) hits |= 1u << (j * kVec + k);
+                    }
+                }
+                if (__ballot_sync(0xffffffffu, hits != 0) == 0) continue;
+                int inc = __popc(hits);
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, inc, d);
+                    if (lane >= d) inc += o;
+                }
                 uint32_t at = 0;
-                if (lane == __ffs(m) - 1) at = atomicAdd(&leader->list_n, __popc(m));
-                at = __shfl_sync(0xffffffffu, at, __ffs(m) - 1) + __popc(m & ((1u << lane) - 1));
-                // sorted ascending: largest value, then lowest index, first
-                if (in) leader->list[at] = ~(static_cast<u64>(key_of(x)) << 32 | (0xffffffffu - (base + i)));
+                if (lane == 31) at = atomicAdd(&leader->list_n, static_cast<uint32_t>(inc));
+                at = __shfl_sync(0xffffffffu, at, 31) + inc - __popc(hits);
+                for (; hits; hits &= hits - 1) {
+                    const int k = __ffs(hits) - 1;
+                    const int i = (v0 + k / kVec * kThreads + tid) * kVec + k % kVec;
+                    // ascending: the largest value, then the lowest index, first
+                    leader->list[at++] = ~(static_cast<u64>(key_of(value(i))) << 32 | (0xffffffffu - (base + i)));
+                }
             }
         };
         if (kept <= kList) {
@@ -346,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             if (rank == 0) {
                 const int cnt = kept, m2 = power_of_two(cnt);
                 for (int i = cnt + tid; i < m2; i += kThreads) s.list[i] = ~0ull;
-                sort_words(s.list, m2);
+                sort_words(s.list, cnt, m2, s.scan32);
                 constexpr int kEach = kList / kThreads;
                 u64 w[kEach], mine_w = 0, kept_w = 0;
 #pragma unroll
@@ -380,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                     if (i < m2) order[i] = i < cnt ? static_cast<u64>(0xffffffffu - at[e]) << 32 | i : ~0ull;
                     w_at[i] = w[e];
                 }
-                sort_words(order, m2);
+                sort_words(order, cnt, m2, s.scan32);
                 u64 o[kEach];
                 mine_w = 0;
 #pragma unroll
@@ -401,6 +482,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             }
             cluster.sync();
             return;
+        }
+
+        // ---- more than that is left: list this CTA's share by index, if it is few
+        cluster.sync();                                   // every CTA has read the counts
+        {
+            uint32_t mine_n = 0;
+            for (int v = first_vec; v < last_vec; ++v) {
+                const uint4 q = xv[v];
+                const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) {
+                    const int b = bin_of(to_float(e[k]));
+                    mine_n += b <= bound && b < kBins - 1;
+                }
+            }
+            uint32_t all_n;
+            uint32_t at = block_inclusive(mine_n, s.scan32, &all_n) - mine_n;
+            if (all_n <= kSparse && p.slice <= 65536) {
+                sparse = all_n;
+                if (mine_n)
+                    for (int v = first_vec; v < last_vec; ++v) {
+                        const uint4 q = xv[v];
+                        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                        for (int k = 0; k < kVec; ++k) {
+                            const int b = bin_of(to_float(e[k]));
+                            if (b <= bound && b < kBins - 1) left[at++] = v * kVec + k;
+                        }
+                    }
+            }
+            __syncthreads();
         }
 
         // ---- the cut bin by bin.  Sum of a count and a weight over the cluster.
@@ -431,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 if (rank == 0) {
                     const int m2 = power_of_two(size);
                     for (int i = size + tid; i < m2; i += kThreads) s.list[i] = ~0ull;
-                    sort_words(s.list, m2);
+                    sort_words(s.list, size, m2, s.scan32);
                     constexpr int kEach = kList / kThreads;
                     u64 w[kEach], mine_w = 0;
 #pragma unroll
@@ -516,8 +628,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             for (int i = tid; i < kBins; i += kThreads) lo[i] = hi[i] = 0;
             // ties at a top-k cut: only cut_ties of them count, all in one bin, of one weight
             __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
-                const float x = value(i);
+            const int walk = sparse >= 0 ? sparse : p.slice;
+            for (int j = tid; j < walk; j += kThreads) {
+                const float x = value(sparse >= 0 ? left[j] : j);
                 const uint32_t key = key_of(x);
                 if (k_on ? key <= cut_key : false) continue;
                 const int b = bin_of(x);
@@ -553,7 +666,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             u64 total;
             const u64 sum4 = wb[0] + wb[1] + wb[2] + wb[3];
             u64 before = block_inclusive(sum4, s.scan, &total) - sum4;
-            const double want_d = ceil(static_cast<double>(share) * static_cast<double>(total));
+            // the bins past the bound were not summed here
+            const u64 whole_w = have_all ? all : total;
+            const double want_d = ceil(static_cast<double>(share) * static_cast<double>(whole_w));
             u64 want = want_d > 1.0 ? static_cast<u64>(want_d) : 1ull;
             if (want > total) want = total;
 #pragma unroll
@@ -572,51 +687,47 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
     }
 
-    // ---- cumulative weights in index order: contiguous pieces per warp
-    const int per = ((n + kWarps - 1) / kWarps + 31) & ~31;
-    const int lo = min(warp * per, n), hi = min(lo + per, n);
-    uint32_t tie_base = 0;
+    // ---- cumulative weights in index order: each thread a contiguous part of the slice, or of
+    // what is listed of it
+    const int each = sparse >= 0 ? (sparse + kThreads - 1) / kThreads : part_vecs * kVec;
+    const int walk = sparse >= 0 ? sparse : p.slice;
+    const int lo = min(tid * each, walk), hi = min(lo + each, walk);
+    auto index = [&](int j) { return sparse >= 0 ? static_cast<int>(left[j]) : j; };
+    uint32_t ties_before = 0;                             // at the cut, before this thread's part
     const bool cut = cut_ties != 0xffffffffu;
     if (cut) {
         uint32_t ties = 0;
-        for (int i = lo + lane; i < hi; i += 32) ties += key_of(value(i)) == cut_key;
-        ties = warp_sum(ties);
-        if (lane == 0) s.warp_ties[warp] = ties;
-        __syncthreads();
-        if (tid == 0) {
-            ties = 0;
-            for (int w = 0; w < kWarps; ++w) ties += s.warp_ties[w];
-            s.ties = ties;
-        }
+        for (int j = lo; j < hi; ++j) ties += key_of(value(index(j))) == cut_key;
+        uint32_t all;
+        ties_before = block_inclusive(ties, s.scan32, &all) - ties;
+        if (tid == 0) s.ties = all;
         cluster.sync();
-        for (int r = 0; r < rank; ++r) tie_base += *cluster.map_shared_rank(&s.ties, r);
-        for (int w = 0; w < warp; ++w) tie_base += s.warp_ties[w];
+        for (int r = 0; r < rank; ++r) ties_before += *cluster.map_shared_rank(&s.ties, r);
     }
-    // kept weight of token i of this warp's piece; `seen` ties lie before the 32 it belongs to
-    auto kept_weight = [&](int i, uint32_t& seen) {
-        const float x = i < hi ? value(i) : 0.0f;
-        const uint32_t key = i < hi ? key_of(x) : 0;
-        bool keep = i < hi && key >= cut_key;
-        if (cut) {
-            const bool tie = i < hi && key == cut_key;
-            const unsigned m = __ballot_sync(0xffffffffu, tie);
-            if (tie) keep = seen + __popc(m & ((1u << lane) - 1)) < cut_ties;
-            seen += __popc(m);
-        }
-        u64 w = keep ? weight(x) : 0;
-        return w >= least_w ? w : 0;
-    };
     u64 sum = 0;
-    uint32_t seen = tie_base;
-    for (int i = lo; i < hi; i += 32) sum += kept_weight(i + lane, seen);
-    sum = warp_sum(sum);
-    if (lane == 0) s.warp_sum[warp] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        sum = 0;
-        for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
-        s.sum = sum;
+    {
+        uint32_t seen = ties_before;
+        auto add = [&](float x) {
+            const uint32_t key = key_of(x);
+            if (key < cut_key) return;
+            if (cut && key == cut_key && seen++ >= cut_ties) return;
+            const u64 w = weight(x);
+            sum += w >= least_w ? w : 0;
+        };
+        if (sparse >= 0) {
+            for (int j = lo; j < hi; ++j) add(value(left[j]));
+        } else {
+            for (int v = first_vec; v < last_vec; ++v) {
+                const uint4 q = xv[v];
+                const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) add(to_float(e[k]));
+            }
+        }
     }
+    u64 mine_total;
+    const u64 inclusive = block_inclusive(sum, s.scan, &mine_total);
+    if (tid == 0) s.sum = mine_total;
     cluster.sync();
     u64 total = 0, before = 0;
     for (int r = 0; r < ctas; ++r) {
@@ -624,22 +735,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         if (r < rank) before += o;
         total += o;
     }
-    for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
     const u64 want = target_of(total);
-    if (before <= want && want < before + s.warp_sum[warp]) {
-        seen = tie_base;
-        for (int i = lo; i < hi; i += 32) {
-            const u64 w = kept_weight(i + lane, seen);
-            u64 inc = w;
+    if (before <= want && want < before + mine_total) {   // the token is in this CTA
+        const u64 upto = before + inclusive;
+        if (upto - sum <= want && want < upto) {          // in this thread's part
+            s.found = lo;
+            s.found_above = ties_before;
+            s.bin_above = upto - sum;
+        }
+        __syncthreads();
+        if (warp == 0) {                                  // 32 tokens of the part at a time
+            const int from = s.found, to = min(from + each, walk);
+            uint32_t seen = s.found_above;
+            u64 at = s.bin_above;
+            for (int j0 = from; j0 < to && at <= want; j0 += 32) {
+                const int j = j0 + lane;
+                const float x = j < to ? value(index(j)) : __int_as_float(0xff800000);
+                const uint32_t key = key_of(x);
+                bool keep = j < to && key >= cut_key;
+                if (cut) {
+                    const unsigned m = __ballot_sync(0xffffffffu, keep && key == cut_key);
+                    if (keep && key == cut_key) keep = seen + __popc(m & ((1u << lane) - 1)) < cut_ties;
+                    seen += __popc(m);
+                }
+                u64 w = keep ? weight(x) : 0;
+                if (w < least_w) w = 0;
+                u64 inc = w;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const u64 o = __shfl_up_sync(0xffffffffu, inc, d);
-                if (lane >= d) inc += o;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const u64 o = __shfl_up_sync(0xffffffffu, inc, d);
+                    if (lane >= d) inc += o;
+                }
+                if (at + inc - w <= want && want < at + inc) p.tokens[row] = base + index(j);
+                at += __shfl_sync(0xffffffffu, inc, 31);
             }
-            const u64 upto = before + inc;
-            if (upto - w <= want && want < upto) p.tokens[row] = base + i + lane;
-            before += __shfl_sync(0xffffffffu, inc, 31);
-            if (before > want) break;
         }
     }
     cluster.sync();
