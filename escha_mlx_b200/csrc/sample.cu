@@ -36,8 +36,10 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCtas = 8;                 // of a row's cluster
 constexpr int kBins = 2048;                 // the last one is not counted: weight 0
 constexpr int kList = 2048;
+constexpr int kByMaxima = 1024;             // largest top-k that is bounded by the threads' maxima
 constexpr int kSparse = 4096;               // listed tokens of a slice (16-bit places over the counts)
 constexpr float kCut = -30.0f;
 constexpr int kFraction = 44;
@@ -112,6 +114,14 @@ struct Weights {
     }
 };
 
+// One word of each CTA of the cluster (0 past the last): the loads are in flight together.
+template <typename V>
+__device__ __forceinline__ void read_ranks(const cg::cluster_group& cluster, V* word, int ctas,
+                                           V (&out)[kMaxCtas]) {
+#pragma unroll
+    for (int r = 0; r < kMaxCtas; ++r) out[r] = r < ctas ? *cluster.map_shared_rank(word, r) : V(0);
+}
+
 template <typename V>
 __device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
@@ -185,6 +195,230 @@ __device__ void sort_words(u64* a, int count, int n, uint32_t* scratch) {
 
 __device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
+// What a row asks of its list.
+struct ListRow {
+    int64_t* token;
+    int k;                                  // 0: no top-k
+    bool p_on;
+    float share;
+    u64 least_w;
+    int V;
+};
+
+// 64-bit sums by bucket, as low and high words (the low one's carry is seen by whoever causes
+// it), and the first bucket at which their running sum exceeds `want`.
+struct Buckets {
+    uint32_t* lo;                           // [kBins]
+    uint32_t* hi;
+    __device__ __forceinline__ void clear() {
+        for (int i = threadIdx.x; i < kBins / 2; i += kThreads)
+            reinterpret_cast<uint4*>(lo)[i] = make_uint4(0, 0, 0, 0);      // lo and hi are neighbours
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add(int b, u64 w) {
+        const uint32_t wl = static_cast<uint32_t>(w);
+        const uint32_t old = atomicAdd(&lo[b], wl);
+        const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + wl < old);
+        if (up) atomicAdd(&hi[b], up);
+    }
+    // found, above: one shared word each, the bucket and the sum before it
+    __device__ __forceinline__ void find(u64 want, u64* scratch, uint32_t* found, u64* above) {
+        __syncthreads();
+        const uint4 l = reinterpret_cast<const uint4*>(lo)[threadIdx.x];
+        const uint4 h = reinterpret_cast<const uint4*>(hi)[threadIdx.x];
+        const u64 w[4] = {(static_cast<u64>(h.x) << 32) + l.x, (static_cast<u64>(h.y) << 32) + l.y,
+                          (static_cast<u64>(h.z) << 32) + l.z, (static_cast<u64>(h.w) << 32) + l.w};
+        u64 total;
+        const u64 mine = w[0] + w[1] + w[2] + w[3];
+        u64 before = block_inclusive(mine, scratch, &total) - mine;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (before <= want && want < before + w[e]) {
+                *found = 4 * threadIdx.x + e;
+                *above = before;
+            }
+            before += w[e];
+        }
+        __syncthreads();
+    }
+};
+
+// Settles a row whose kept tokens are all among the `count` of s.list (any order, as
+// ~(key, ~index)), by one CTA.  `all`: weight of the whole row, 0: that of the list (its first
+// k).  Each cut is found by buckets (bins of d, then ranges of the index), exactly inside the
+// one bucket where it falls; up to kCounted tokens are compared all with all instead.
+template <class W, class B, class G>
+__device__ void settle_list(Shared& s, int count, const ListRow& r, const W& weight, const B& bin_of,
+                            const G& target_of, u64 all) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (count <= kCounted) {
+        // kThreads / m threads per token, at most a warp
+        const int m = power_of_two(count), per = min(32, kThreads / m), i = tid / per, part = tid % per;
+        u64* ws = reinterpret_cast<u64*>(s.cum);          // weights by rank, then the kept ones
+        int* at = reinterpret_cast<int*>(s.cum + 2 * kCounted);
+        const u64 x = i < count ? s.list[i] : 0;
+        int ahead = 0;
+        if (i < count)
+            for (int j = part; j < count; j += per) ahead += s.list[j] < x;
+        for (int d = 1; d < per; d <<= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+        const int index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(~x));
+        if (i < count && part == 0) {
+            ws[ahead] = weight(value_of(static_cast<uint32_t>(~x >> 32)));
+            at[ahead] = index;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            constexpr int kEach = kCounted / 32;
+            u64 w[kEach], mine = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int j = lane * kEach + e;
+                w[e] = j < count && (r.k == 0 || j < r.k) ? ws[j] : 0;
+                mine += w[e];
+            }
+            u64 inc = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const u64 o = __shfl_up_sync(0xffffffffu, inc, d);
+                if (lane >= d) inc += o;
+            }
+            u64 before = inc - mine;
+            const u64 total = __shfl_sync(0xffffffffu, inc, 31);
+            const double want = static_cast<double>(r.share) * static_cast<double>(all ? all : total);
+            mine = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int j = lane * kEach + e;
+                const bool keep = w[e] >= r.least_w && (!r.p_on || j == 0 || static_cast<double>(before) < want);
+                before += w[e];
+                if (!keep) w[e] = 0;
+                if (j < count) ws[j] = w[e];
+                mine += w[e];
+            }
+            mine = warp_sum(mine);
+            if (lane == 0) s.bin_above = target_of(mine);
+        }
+        __syncthreads();
+        const u64 want = s.bin_above;
+        u64 upto = 0;
+        if (i < count)
+            for (int j = part; j < count; j += per) upto += at[j] <= index ? ws[j] : 0;
+        for (int d = 1; d < per; d <<= 1) upto += __shfl_xor_sync(0xffffffffu, upto, d);
+        if (i < count && part == 0 && upto - ws[ahead] <= want && want < upto) *r.token = index;
+        return;
+    }
+
+    constexpr int kEach = kList / kThreads;
+    u64 x[kEach], w[kEach];
+    int bin[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = tid + e * kThreads;
+        x[e] = i < count ? s.list[i] : ~0ull;
+        const float v = value_of(static_cast<uint32_t>(~x[e] >> 32));
+        bin[e] = i < count ? bin_of(v) : kBins;
+        w[e] = i < count ? weight(v) : 0;
+    }
+    __syncthreads();
+    Buckets b{s.hist, s.cum};
+    // Tokens of a bucket, by a key to sort by (ascending), in the list's place, their weights in
+    // the buckets'; returns how many.
+    u64* const ws = reinterpret_cast<u64*>(s.hist);
+    auto collect = [&](int bucket, const int (&of)[kEach], const u64 (&key)[kEach]) {
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (of[e] == bucket && w[e] != 0) {
+                const uint32_t at = atomicAdd(&s.count, 1u);
+                s.list[at] = key[e];
+                ws[at] = w[e];
+            }
+        __syncthreads();
+        return static_cast<int>(s.count);
+    };
+    // The key in a collected bucket at which the running sum of `unit ? 1 : weight` exceeds `want`.
+    auto settle = [&](int n, u64 want, bool unit) {
+        const int per = n <= 16 ? 32 : n <= kCounted ? kThreads / power_of_two(n) : 1;
+        for (int i = tid / per; i < n; i += kThreads / per) {
+            // every thread of a group runs the same rounds; groups lie within a warp
+            const u64 key = s.list[i], mine = unit ? 1 : ws[i];
+            u64 before = 0;
+            for (int j = tid % per; j < n; j += per)
+                if (s.list[j] < key) before += unit ? 1 : ws[j];
+            const unsigned group = per == 32 ? 0xffffffffu : ((1u << per) - 1) << (lane / per * per);
+            for (int d = 1; d < per; d <<= 1) before += __shfl_xor_sync(group, before, d);
+            if (before <= want && want < before + mine) s.best = key;
+        }
+        __syncthreads();
+        return s.best;
+    };
+    auto sum_of = [&]() {
+        u64 mine = 0, total;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) mine += w[e];
+        block_inclusive(mine, s.scan, &total);
+        return total;
+    };
+    if (r.k > 0) {
+        int some = 0, all_some;                           // tokens that weigh something
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) some += w[e] != 0;
+        block_inclusive(some, reinterpret_cast<int*>(s.scan32), &all_some);
+        if (r.k < all_some) {
+            b.clear();
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                if (w[e] != 0) atomicAdd(&b.lo[bin[e]], 1u);
+            b.find(r.k - 1, s.scan, &s.found, &s.bin_above);
+            const u64 above = s.bin_above;
+            const int n = collect(s.found, bin, x);
+            const u64 cut = settle(n, r.k - 1 - above, true);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                if (x[e] > cut) w[e] = 0;
+        }
+    }
+    if (r.p_on) {
+        const u64 total = sum_of();
+        // kept while the sum before a token is below share * total: up to the first token at
+        // which the running sum exceeds the last whole number below that
+        const double want_d = ceil(static_cast<double>(r.share) * static_cast<double>(all ? all : total)) - 1.0;
+        u64 want = want_d > 0.0 ? static_cast<u64>(want_d) : 0ull;
+        if (want > total - 1) want = total - 1;
+        b.clear();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (w[e] != 0) b.add(bin[e], w[e]);
+        b.find(want, s.scan, &s.found, &s.bin_above);
+        const u64 above = s.bin_above;
+        const int n = collect(s.found, bin, x);
+        const u64 cut = settle(n, want - above, false);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (x[e] > cut) w[e] = 0;
+    }
+    u64 index[kEach];
+    int range[kEach];
+    const int shift = max(0, 32 - __clz(r.V - 1) - 11);   // 2048 ranges of indices
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if (w[e] < r.least_w) w[e] = 0;
+        index[e] = 0xffffffffu - static_cast<uint32_t>(~x[e]);
+        range[e] = w[e] != 0 ? static_cast<int>(index[e] >> shift) : kBins;
+    }
+    const u64 want = target_of(sum_of());
+    b.clear();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (w[e] != 0) b.add(range[e], w[e]);
+    b.find(want, s.scan, &s.found, &s.bin_above);
+    const u64 above = s.bin_above;
+    const int n = collect(s.found, range, index);
+    const u64 token = settle(n, want - above, false);
+    if (tid == 0) *r.token = static_cast<int64_t>(token);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -231,18 +465,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             for (int k = 0; k < kVec; ++k) take(v * kVec + k, e[k]);
         }
     }
-    for (int i0 = whole * kVec + tid; i0 < p.slice; i0 += 2 * kBatch * kThreads) {
+    const int head_of_rest = whole * kVec;                // the rest, token by token
+    for (int i0 = head_of_rest + tid; i0 < p.slice; i0 += 2 * kBatch * kThreads) {
         T q[2 * kBatch];
 #pragma unroll
         for (int j = 0; j < 2 * kBatch; ++j)
             q[j] = i0 + j * kThreads < n ? src[i0 + j * kThreads] : lowest<T>();
 #pragma unroll
-        for (int j = 0; j < 2 * kBatch; ++j) {
-            const int i = i0 + j * kThreads;
-            if (i >= p.slice) break;
-            xs[i] = q[j];
-            take(i, q[j]);
-        }
+        for (int j = 0; j < 2 * kBatch; ++j)
+            if (i0 + j * kThreads < p.slice) xs[i0 + j * kThreads] = q[j];
+    }
+    __syncthreads();
+    // a thread's maximum is over the vectors that it owns in every later pass too
+    for (int v = whole + (tid + kThreads - whole % kThreads) % kThreads; v < vecs; v += kThreads) {
+        const uint4 q = xv[v];
+        const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) take(v * kVec + k, e[k]);
     }
     u64 best = static_cast<u64>(key_of(most)) << 32 | (0xffffffffu - (base + most_at));
 #pragma unroll
@@ -260,9 +499,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
     cluster.sync();
     best = 0;
-    for (int r = 0; r < ctas; ++r) {
-        const u64 o = *cluster.map_shared_rank(&s.best, r);
-        best = o > best ? o : best;
+    {
+        u64 o[kMaxCtas];
+        read_ranks(cluster, &s.best, ctas, o);
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) best = o[r] > best ? o[r] : best;
     }
     const float top = value_of(static_cast<uint32_t>(best >> 32));
     const int top_index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
@@ -311,6 +552,117 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     // ---- the cut: kept are keys above cut_key and the first cut_ties (by index) at it
     uint32_t cut_key = 0, cut_ties = 0xffffffffu;
     if (k_on || p_on || m_on) {
+        Shared* leader = cluster.map_shared_rank(&s, 0);
+        const int my_bin = bin_of(most);                  // the first bin among this thread's tokens
+        // tokens of bins [from, to] to the leader's list (as far as it has room)
+        auto gather = [&](int from, int to) {
+            if (__ballot_sync(0xffffffffu, my_bin <= to) == 0) return;
+            // 64 tokens per thread and round: their hits as a mask, one reservation per warp
+            constexpr int kRound = 64 / kVec;
+            for (int v0 = 0; v0 < vecs; v0 += kRound * kThreads) {
+                u64 hits = 0;
+                if (my_bin <= to) {
+#pragma unroll
+                    for (int j = 0; j < kRound; ++j) {
+                        const int v = v0 + j * kThreads + tid;
+                        if (v >= vecs) break;
+                        const uint4 q = xv[v];
+                        const T* e = reinterpret_cast<const T*>(&q);
+                        unsigned some = 0;
+#pragma unroll
+                        for (int k = 0; k < kVec; ++k) {
+                            const int b = bin_of(to_float(e[k]));
+                            if (b >= from && b <= to && b < kBins - 1) some |= 1u << k;
+                        }
+                        hits |= static_cast<u64>(some) << (j * kVec);
+                    }
+                }
+                if (__ballot_sync(0xffffffffu, hits != 0) == 0) continue;
+                int inc = __popcll(hits);
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, inc, d);
+                    if (lane >= d) inc += o;
+                }
+                uint32_t at = 0;
+                if (lane == 31) at = atomicAdd(&leader->list_n, static_cast<uint32_t>(inc));
+                at = __shfl_sync(0xffffffffu, at, 31) + inc - __popcll(hits);
+                for (; hits; hits &= hits - 1, ++at) {
+                    const int k = __ffsll(hits) - 1;
+                    const int i = (v0 + k / kVec * kThreads + tid) * kVec + k % kVec;
+                    // ascending: the largest value, then the lowest index, first
+                    if (at < kList)
+                        leader->list[at] = ~(static_cast<u64>(key_of(value(i))) << 32 | (0xffffffffu - (base + i)));
+                }
+            }
+        };
+        // counts of the row by bin, from those of the CTAs: an inclusive prefix in s.cum, the
+        // thread's four bins in c, its prefix before them returned
+        uint4 c;
+        uint32_t counted;
+        auto merge = [&]() {
+            uint4 o[kMaxCtas];
+#pragma unroll
+            for (int r = 0; r < kMaxCtas; ++r)
+                o[r] = r < ctas ? reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.hist, r))[tid]
+                                : make_uint4(0, 0, 0, 0);
+            c = o[0];
+#pragma unroll
+            for (int r = 1; r < kMaxCtas; ++r) {
+                c.x += o[r].x; c.y += o[r].y; c.z += o[r].z; c.w += o[r].w;
+            }
+            const uint32_t mine = c.x + c.y + c.z + c.w;
+            const uint32_t before = block_inclusive(mine, s.scan32, &counted) - mine;
+            reinterpret_cast<uint4*>(s.cum)[tid] =
+                make_uint4(before + c.x, before + c.x + c.y, before + c.x + c.y + c.z, before + mine);
+            if (tid == 0) s.found = kBins - 1;
+            __syncthreads();
+            return before;
+        };
+        // the bin in which the count-th token lies (all bins: not among the counted)
+        auto bin_of_count = [&](uint32_t before, uint32_t count) {
+            if (before < count && count <= before + c.x + c.y + c.z + c.w) {
+                count -= before;
+                s.found = 4 * tid + (count <= c.x ? 0 : count <= c.x + c.y ? 1
+                                     : count <= c.x + c.y + c.z ? 2 : 3);
+            }
+            __syncthreads();
+            return static_cast<int>(s.found);
+        };
+        int m_bin = kBins - 1;
+        if (m_on) m_bin = min(kBins - 1, static_cast<int>((-logf(least) + 1e-3f) * kBinsPerNat));
+        const ListRow row_of{p.tokens + row, k_on ? k : 0, p_on, share, least_w, p.V};
+
+        if (k_on && k <= kByMaxima) {
+            // ---- a small top-k: the count-th largest of the threads' maxima is a lower bound
+            // of the count-th largest token, and nearly as large where k is far fewer than the
+            // threads; only the maxima are counted (all tokens: 5 us of shared-memory atomics)
+            if (my_bin < kBins - 1) atomicAdd(&s.hist[my_bin], 1u);
+            cluster.sync();
+            const uint32_t before = merge();
+            if (static_cast<uint32_t>(k) <= counted) {
+                const int k_bin = bin_of_count(before, k);
+                gather(0, p_on ? k_bin : min(k_bin, m_bin));
+                cluster.sync();
+                const uint32_t got = leader->list_n;
+                if (got <= kList) {
+                    if (rank == 0) settle_list(s, static_cast<int>(got), row_of, weight, bin_of, target_of, 0);
+                    cluster.sync();
+                    return;
+                }
+            }
+            cluster.sync();                               // all have read the counts and list_n
+            if (rank == 0 && tid == 0) s.list_n = 0;
+            for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
+            __syncthreads();
+        }
+
+        // ---- counts of all tokens by bin, as far as they can matter: without top-k, those that
+        // weigh less than (1 - p) / V of the largest together weigh less than top-p leaves out
+        int last = kBins - 1;
+        if (p_on && !k_on)
+            last = min(last, static_cast<int>((logf(static_cast<float>(p.V) / (1.0f - share)) + 1e-2f) * kBinsPerNat) + 1);
+        if (!k_on) last = min(last, m_bin + 1);
         u64 sum = 0;
         for (int v = tid; v < vecs; v += kThreads) {
             const uint4 q = xv[v];
@@ -318,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 #pragma unroll
             for (int k = 0; k < kVec; ++k) {
                 const int b = bin_of(to_float(e[k]));
-                if (b < kBins - 1) atomicAdd(&s.hist[b], 1u);
+                if (b < last) atomicAdd(&s.hist[b], 1u);
             }
             if (p_on && !k_on)
 #pragma unroll
@@ -333,36 +685,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             s.sum = sum;
         }
         cluster.sync();
-        u64 all = 0;                                      // weight of the row (p_on && !k_on)
-        uint4 c = make_uint4(0, 0, 0, 0);                 // bins 4 tid .. 4 tid + 3
-        for (int r = 0; r < ctas; ++r) {
-            const uint4 o = reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.hist, r))[tid];
-            c.x += o.x; c.y += o.y; c.z += o.z; c.w += o.w;
-            all += *cluster.map_shared_rank(&s.sum, r);
+        u64 all = 0;                                      // weight of the row (p_on without top-k)
+        {
+            u64 o[kMaxCtas];
+            read_ranks(cluster, &s.sum, ctas, o);
+#pragma unroll
+            for (int r = 0; r < kMaxCtas; ++r) all += o[r];
         }
-        uint32_t counted;
-        const uint32_t mine = c.x + c.y + c.z + c.w;
-        const uint32_t inc = block_inclusive(mine, s.scan32, &counted);
-        const uint32_t c0 = inc - mine + c.x, c1 = c0 + c.y, c2 = c1 + c.z;
-        reinterpret_cast<uint4*>(s.cum)[tid] = make_uint4(c0, c1, c2, inc);
+        const uint32_t before_bins = merge();
+        // without top-k; a top-k that turns out to cut nothing takes the exact way below
+        const bool have_all = p_on && !k_on;
         // tokens past the counted bins weigh nothing, so a top-k that reaches them cuts nothing
         k_on = k_on && static_cast<uint32_t>(k) <= counted;
-        if (tid == 0) s.found = kBins - 1;
-        __syncthreads();
-        int k_bin = kBins - 1;
-        if (k_on) {
-            const uint32_t kk = k;
-            if (inc - mine < kk && kk <= inc)
-                s.found = 4 * tid + (kk <= c0 ? 0 : kk <= c1 ? 1 : kk <= c2 ? 2 : 3);
-            __syncthreads();
-            k_bin = s.found;
-        }
-        int m_bin = kBins - 1;
-        if (m_on) m_bin = min(kBins - 1, static_cast<int>((-logf(least) + 1e-3f) * kBinsPerNat));
-        int p_bin = kBins - 1;
-        // the weight of the row was summed only without top-k; a top-k that turned out to cut
-        // nothing takes the exact way below
-        const bool have_all = p_on && !(k > 0 && k < p.V);
+        const int k_bin = k_on ? bin_of_count(before_bins, k) : kBins - 1;
+        int p_bin = last - 1;
         if (have_all) {
             // least weight that a bin's tokens can have, less a thousandth for rounding
             auto low = [](int b) { return exp2f((b + 1) * (-1.44269504f / kBinsPerNat)) * 0.999f; };
@@ -371,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             float total;
             const float before = block_inclusive(w3, s.scanf, &total) - w3;
             const float want = share * (static_cast<float>(all) * 0x1p-44f) * 1.0001f;
-            if (tid == 0) s.found = kBins - 1;
+            if (tid == 0) s.found = last - 1;
             __syncthreads();
             if (before + w3 >= want) {                    // the first such bin
                 const int b = 4 * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
@@ -384,101 +720,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         const int bound = k_on ? (p_on ? k_bin : min(k_bin, m_bin)) : p_on && !have_all ? kBins - 1
                                                                       : min(p_bin, m_bin);
         const uint32_t kept = s.cum[bound];
-        Shared* leader = cluster.map_shared_rank(&s, 0);
-        // tokens of bins [from, to] to the leader's list
-        auto gather = [&](int from, int to) {
-            // 32 tokens per thread and round: their hits as a mask, one reservation per warp
-            constexpr int kRound = 32 / kVec;
-            for (int v0 = 0; v0 < vecs; v0 += kRound * kThreads) {
-                unsigned hits = 0;
-#pragma unroll
-                for (int j = 0; j < kRound; ++j) {
-                    const int v = v0 + j * kThreads + tid;
-                    const uint4 q = v < vecs ? xv[v] : make_uint4(0, 0, 0, 0);
-                    const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-                    for (int k = 0; k < kVec; ++k) {
-                        const int b = bin_of(to_float(e[k]));
-                        if (v < vecs && b >= from && b <= to && b < kBins - 1) hits |= 1u << (j * kVec + k);
-                    }
-                }
-                if (__ballot_sync(0xffffffffu, hits != 0) == 0) continue;
-                int inc = __popc(hits);
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int o = __shfl_up_sync(0xffffffffu, inc, d);
-                    if (lane >= d) inc += o;
-                }
-                uint32_t at = 0;
-                if (lane == 31) at = atomicAdd(&leader->list_n, static_cast<uint32_t>(inc));
-                at = __shfl_sync(0xffffffffu, at, 31) + inc - __popc(hits);
-                for (; hits; hits &= hits - 1) {
-                    const int k = __ffs(hits) - 1;
-                    const int i = (v0 + k / kVec * kThreads + tid) * kVec + k % kVec;
-                    // ascending: the largest value, then the lowest index, first
-                    leader->list[at++] = ~(static_cast<u64>(key_of(value(i))) << 32 | (0xffffffffu - (base + i)));
-                }
-            }
-        };
         if (kept <= kList) {
             // ---- everything that can be kept fits the list: one CTA settles the row
             gather(0, bound);
             cluster.sync();
             if (rank == 0) {
-                const int cnt = kept, m2 = power_of_two(cnt);
-                for (int i = cnt + tid; i < m2; i += kThreads) s.list[i] = ~0ull;
-                sort_words(s.list, cnt, m2, s.scan32);
-                constexpr int kEach = kList / kThreads;
-                u64 w[kEach], mine_w = 0, kept_w = 0;
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int i = tid * kEach + e;
-                    w[e] = i < cnt ? weight(value_of(static_cast<uint32_t>(~s.list[i] >> 32))) : 0;
-                    if (k_on && i >= k) w[e] = 0;
-                    mine_w += w[e];
-                }
-                u64 total;
-                u64 before = block_inclusive(mine_w, s.scan, &total) - mine_w;
-                const double want = static_cast<double>(share) * static_cast<double>(have_all ? all : total);
-                uint32_t at[kEach];
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int i = tid * kEach + e;
-                    bool keep = i < cnt && w[e] != 0 && w[e] >= least_w;
-                    if (p_on) keep = keep && (i == 0 || static_cast<double>(before) < want);
-                    before += w[e];
-                    if (!keep) w[e] = 0;
-                    kept_w += w[e];
-                    at[e] = i < cnt ? static_cast<uint32_t>(~s.list[i]) : 0;     // ~index
-                }
-                block_inclusive(kept_w, s.scan, &total);
-                // cumulative weights in index order: sort by index, carrying the position
-                u64* order = s.list;
-                u64* w_at = reinterpret_cast<u64*>(s.hist);        // hist and cum: 2048 words
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int i = tid * kEach + e;
-                    if (i < m2) order[i] = i < cnt ? static_cast<u64>(0xffffffffu - at[e]) << 32 | i : ~0ull;
-                    w_at[i] = w[e];
-                }
-                sort_words(order, cnt, m2, s.scan32);
-                u64 o[kEach];
-                mine_w = 0;
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int i = tid * kEach + e;
-                    o[e] = i < cnt ? order[i] : 0;
-                    w[e] = i < cnt ? w_at[static_cast<uint32_t>(o[e])] : 0;
-                    mine_w += w[e];
-                }
-                u64 again;
-                before = block_inclusive(mine_w, s.scan, &again) - mine_w;
-                const u64 want_u = target_of(total);
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    if (before <= want_u && want_u < before + w[e]) p.tokens[row] = static_cast<int>(o[e] >> 32);
-                    before += w[e];
-                }
+                ListRow r = row_of;
+                if (!k_on) r.k = 0;
+                settle_list(s, static_cast<int>(kept), r, weight, bin_of, target_of, have_all ? all : 0);
             }
             cluster.sync();
             return;
