@@ -40,9 +40,11 @@ constexpr int kMaxCtas = 8;                 // of a row's cluster
 constexpr int kBins = 2048;                 // the last one is not counted: weight 0
 constexpr int kList = 2048;
 constexpr int kByMaxima = 1024;             // largest top-k that is bounded by the threads' maxima
+constexpr int kNear = 5;                    // bins around where a top-p cut is expected
 constexpr int kSparse = 4096;               // listed tokens of a slice (16-bit places over the counts)
 constexpr float kCut = -30.0f;
 constexpr int kFraction = 44;
+static_assert(kThreads == 512, "one thread per entry of the table of powers");
 constexpr float kBinsPerNat = (kBins - 1) / 30.25f;
 typedef unsigned long long u64;
 
@@ -66,7 +68,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 struct Shared {
-    double pow2[32];                        // 2^(j / 32)
+    double pow2[512];                       // 2^(j / 512)
     u64 best;                               // this CTA's largest (key, ~index)
     u64 sum;                                // this CTA's sum of weights
     u64 warp_sum[kWarps];
@@ -81,34 +83,33 @@ struct Shared {
     uint32_t cut_key;                       // (leader) the cut, for all CTAs
     uint32_t cut_ties;
     u64 bin_above;
+    u64 near[kNear + 2];                    // weights of the bins around a cut, before and behind
     __align__(16) uint32_t hist[kBins];     // counts of this CTA
     __align__(16) uint32_t cum[kBins];      // counts of the row, inclusive prefix
     __align__(16) u64 list[kList];          // (leader) tokens as (key, ~index); or per-bin weights
 };
 
-// Weight of a token in units of 2^-44.  2^(y / 32) = 2^(n / 32) * exp(r): a table for the
-// 32nds, a Taylor series of degree 5 for |r| <= ln 2 / 64 (remainder below 3e-15).
+// Weight of a token in units of 2^-44.  2^(y / 512) = 2^(n / 512) * exp(r): a table for the
+// 512ths, a Taylor series of degree 3 for |r| <= ln 2 / 1024 (remainder below 9e-15).
 struct Weights {
-    double top, inv;
+    double top, inv, inv512;                // 1 / T, and that times 512 log2(e)
     float topf;
     const double* pow2;
     __device__ __forceinline__ u64 operator()(float x) const {
         if (x == topf) return 1ull << kFraction;
-        const double d = (static_cast<double>(x) - top) * inv;
-        if (!(d >= static_cast<double>(kCut))) return 0;
-        const double y = d * 46.166241308446828384;                  // 32 log2(e)
+        const double d = static_cast<double>(x) - top;
+        if (!(d * inv >= static_cast<double>(kCut))) return 0;
+        const double y = d * inv512;
         const double magic = 6755399441055744.0;                     // 1.5 * 2^52: rounds to integer
         const double shifted = y + magic;
         const int n = static_cast<int>(__double_as_longlong(shifted));
-        const double r = (y - (shifted - magic)) * 0.021660849392498290;   // ln 2 / 32
-        double e = 1.0 / 120.0;
-        e = fma(e, r, 1.0 / 24.0);
-        e = fma(e, r, 1.0 / 6.0);
-        e = fma(e, r, 0.5);
+        const double r = y - (shifted - magic);
+        constexpr double c = 0.0013538030870311433;                  // ln 2 / 512
+        double e = fma(c * c * c / 6.0, r, c * c / 2.0);
+        e = fma(e, r, c);
         e = fma(e, r, 1.0);
-        e = fma(e, r, 1.0);
-        const long long scale = static_cast<long long>((n >> 5) + kFraction) << 52;
-        const double t = __longlong_as_double(__double_as_longlong(pow2[n & 31]) + scale);
+        const long long scale = static_cast<long long>((n >> 9) + kFraction) << 52;
+        const double t = __longlong_as_double(__double_as_longlong(pow2[n & 511]) + scale);
         // t * e <= 2^44: adding 2^52 leaves the nearest integer in the low mantissa bits
         return static_cast<u64>(__double_as_longlong(fma(t, e, 4503599627370496.0))) & 0xfffffffffffffull;
     }
@@ -429,9 +430,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const int row = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_launch_dependents();
-    if (tid < 32) s.pow2[tid] = exp2(tid / 32.0);
+    s.pow2[tid] = exp2(tid / 512.0);
     if (tid == 0) s.list_n = 0;
     grid_dependency_wait();
+
+    // settings of the row, on their way while the logits are read
+    const float temperature = p.temperature ? p.temperature[row] : p.temperature1;
+    const int k = p.top_k ? p.top_k[row] : p.top_k1;
+    const float share0 = p.top_p ? p.top_p[row] : p.top_p1;
+    const float least0 = p.min_p ? p.min_p[row] : p.min_p1;
+    const float u = p.uniforms[row];
 
     // ---- the CTA's slice (filled up with -inf), and the row's maximum with its lowest index
     const int base = rank * p.slice;
@@ -507,25 +515,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     const float top = value_of(static_cast<uint32_t>(best >> 32));
     const int top_index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
-    const float temperature = p.temperature ? p.temperature[row] : p.temperature1;
     const bool empty = top == __int_as_float(0xff800000);
     if (empty || !(temperature > 0.0f)) {
         if (rank == 0 && tid == 0) p.tokens[row] = empty ? -1 : top_index;
         cluster.sync();                     // no CTA leaves while its memory is read
         return;
     }
-    const int k = p.top_k ? p.top_k[row] : p.top_k1;
-    const float share = fmaxf(p.top_p ? p.top_p[row] : p.top_p1, 0.0f);
-    const float least = fminf(p.min_p ? p.min_p[row] : p.min_p1, 1.0f);
-    const float u = p.uniforms[row];
+    const float share = fmaxf(share0, 0.0f), least = fminf(least0, 1.0f);
     bool k_on = k > 0 && k < p.V;
-    const bool p_on = (p.top_p ? p.top_p[row] : p.top_p1) < 1.0f, m_on = least > 0.0f;
+    const bool p_on = share0 < 1.0f, m_on = least > 0.0f;
     const u64 least_w = m_on ? static_cast<u64>(ceil(static_cast<double>(least) * (1ull << kFraction))) : 0;
 
     Weights weight;
     weight.top = top;
     weight.topf = top;
     weight.inv = 1.0 / static_cast<double>(temperature);
+    weight.inv512 = weight.inv * 738.65986093514925;      // 512 log2(e)
     weight.pow2 = s.pow2;
     const float invf = 1.0f / temperature;
     auto value = [&](int i) { return to_float(xs[i]); };
@@ -548,6 +553,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     // tokens of the slice that can be kept, by index (over the counts); -1: not listed
     uint16_t* const left = reinterpret_cast<uint16_t*>(s.hist);
     int sparse = -1;
+    // bins around a top-p cut, and this part's kept weight in those before them
+    int near_lo = -1, near_hi = -1;
+    u64 kept_ahead = 0;
 
     // ---- the cut: kept are keys above cut_key and the first cut_ties (by index) at it
     uint32_t cut_key = 0, cut_ties = 0xffffffffu;
@@ -663,7 +671,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         if (p_on && !k_on)
             last = min(last, static_cast<int>((logf(static_cast<float>(p.V) / (1.0f - share)) + 1e-2f) * kBinsPerNat) + 1);
         if (!k_on) last = min(last, m_bin + 1);
-        u64 sum = 0;
         for (int v = tid; v < vecs; v += kThreads) {
             const uint4 q = xv[v];
             const T* e = reinterpret_cast<const T*>(&q);
@@ -672,62 +679,67 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 const int b = bin_of(to_float(e[k]));
                 if (b < last) atomicAdd(&s.hist[b], 1u);
             }
-            if (p_on && !k_on)
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) sum += weight(to_float(e[k]));
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) s.warp_sum[warp] = sum;
-        __syncthreads();
-        if (tid == 0) {
-            sum = 0;
-            for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
-            s.sum = sum;
         }
         cluster.sync();
-        u64 all = 0;                                      // weight of the row (p_on without top-k)
-        {
-            u64 o[kMaxCtas];
-            read_ranks(cluster, &s.sum, ctas, o);
-#pragma unroll
-            for (int r = 0; r < kMaxCtas; ++r) all += o[r];
-        }
         const uint32_t before_bins = merge();
-        // without top-k; a top-k that turns out to cut nothing takes the exact way below
-        const bool have_all = p_on && !k_on;
         // tokens past the counted bins weigh nothing, so a top-k that reaches them cuts nothing
         k_on = k_on && static_cast<uint32_t>(k) <= counted;
         const int k_bin = k_on ? bin_of_count(before_bins, k) : kBins - 1;
-        int p_bin = last - 1;
-        if (have_all) {
-            // least weight that a bin's tokens can have, less a thousandth for rounding
+        // Top-p without top-k: the bins' weights lie within 1.5% (a thousandth for rounding), so
+        // the cut is surely not past p_bin, and probably within two bins of p_near.
+        int p_bin = last - 1, p_near = 0;
+        if (p_on && !k_on) {
             auto low = [](int b) { return exp2f((b + 1) * (-1.44269504f / kBinsPerNat)) * 0.999f; };
+            constexpr float kHigh = 1.018f;               // top of a bin over its low
             const float w0 = c.x * low(4 * tid), w1 = w0 + c.y * low(4 * tid + 1);
             const float w2 = w1 + c.z * low(4 * tid + 2), w3 = w2 + c.w * low(4 * tid + 3);
             float total;
             const float before = block_inclusive(w3, s.scanf, &total) - w3;
-            const float want = share * (static_cast<float>(all) * 0x1p-44f) * 1.0001f;
-            if (tid == 0) s.found = last - 1;
-            __syncthreads();
-            if (before + w3 >= want) {                    // the first such bin
-                const int b = 4 * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
-                                         : before + w2 >= want ? 2 : 3);
-                atomicMin(&s.found, static_cast<uint32_t>(b));
-            }
-            __syncthreads();
-            p_bin = s.found;
+            // the first bin at which the running sum reaches `want`
+            auto first = [&](float want) {
+                if (tid == 0) s.found = last - 1;
+                __syncthreads();
+                if (before + w3 >= want)
+                    atomicMin(&s.found, 4u * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
+                                                    : before + w2 >= want ? 2 : 3));
+                __syncthreads();
+                const int b = s.found;
+                __syncthreads();
+                return b;
+            };
+            // tokens that were not counted weigh 1 - share at most
+            p_bin = first(share * (total * kHigh + (1.0f - share)) * 1.0001f);
+            p_near = first(share * total);
         }
-        const int bound = k_on ? (p_on ? k_bin : min(k_bin, m_bin)) : p_on && !have_all ? kBins - 1
-                                                                      : min(p_bin, m_bin);
+        const int bound = k_on ? (p_on ? k_bin : min(k_bin, m_bin)) : min(p_bin, m_bin);
         const uint32_t kept = s.cum[bound];
         if (kept <= kList) {
             // ---- everything that can be kept fits the list: one CTA settles the row
             gather(0, bound);
+            u64 sum = 0;
+            if (p_on && !k_on) {                          // top-p asks for the weight of the row
+                for (int v = tid; v < vecs; v += kThreads) {
+                    const uint4 q = xv[v];
+                    const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                    for (int k = 0; k < kVec; ++k) sum += weight(to_float(e[k]));
+                }
+                u64 mine;
+                block_inclusive(sum, s.scan, &mine);
+                if (tid == 0) s.sum = mine;
+            }
             cluster.sync();
             if (rank == 0) {
+                u64 all = 0;
+                if (p_on && !k_on) {
+                    u64 o[kMaxCtas];
+                    read_ranks(cluster, &s.sum, ctas, o);
+#pragma unroll
+                    for (int r = 0; r < kMaxCtas; ++r) all += o[r];
+                }
                 ListRow r = row_of;
                 if (!k_on) r.k = 0;
-                settle_list(s, static_cast<int>(kept), r, weight, bin_of, target_of, have_all ? all : 0);
+                settle_list(s, static_cast<int>(kept), r, weight, bin_of, target_of, all);
             }
             cluster.sync();
             return;
@@ -735,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 
         // ---- more than that is left: list this CTA's share by index, if it is few
         cluster.sync();                                   // every CTA has read the counts
-        {
+        if (k_on || !p_on) {
             uint32_t mine_n = 0;
             for (int v = first_vec; v < last_vec; ++v) {
                 const uint4 q = xv[v];
@@ -870,54 +882,113 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             const uint32_t above = k_bin ? s.cum[k_bin - 1] : 0;
             cut_in_bin(k_bin, s.cum[k_bin] - above, true, k - above, 0);
         }
-        if (p_on) {
-            // exact weights per bin of what is kept so far: low and high words with a carry
+        bool settled = !p_on;
+        if (p_on && !k_on) {
+            // One pass over the tokens (each thread its part in index order): the exact weights
+            // of the bins before the cut's neighbourhood, of each bin in it and of those behind.
+            near_lo = max(p_near - 2, 0);
+            near_hi = min(p_near + 2, last - 1);
             uint32_t* lo = reinterpret_cast<uint32_t*>(s.list);
-            uint32_t* hi = lo + kBins;
-            for (int i = tid; i < kBins; i += kThreads) lo[i] = hi[i] = 0;
-            // ties at a top-k cut: only cut_ties of them count, all in one bin, of one weight
+            if (tid < 2 * kNear) lo[tid] = 0;
             __syncthreads();
+            u64 ahead = 0, behind = 0;
+            for (int v = first_vec; v < last_vec; ++v) {
+                const uint4 q = xv[v];
+                const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) {
+                    const float x = to_float(e[k]);
+                    const int b = bin_of(x);
+                    if (b >= kBins - 1) continue;
+                    const u64 w = weight(x);
+                    if (b < near_lo) {
+                        ahead += w;
+                        kept_ahead += w >= least_w ? w : 0;
+                    } else if (b > near_hi) {
+                        behind += w;
+                    } else {
+                        Buckets{lo, lo + kNear}.add(b - near_lo, w);
+                    }
+                }
+            }
+            u64 mine;
+            block_inclusive(ahead, s.scan, &mine);
+            if (tid == 0) s.near[kNear] = mine;
+            block_inclusive(behind, s.scan, &mine);       // its barriers also end the bins' sums
+            if (tid == 0) s.near[kNear + 1] = mine;
+            if (tid < kNear) s.near[tid] = (static_cast<u64>(lo[kNear + tid]) << 32) + lo[tid];
+            cluster.sync();
+            u64* sums = s.list + kNear;                   // past the words above
+            if (tid < kNear + 2) {
+                u64 o[kMaxCtas], t = 0;
+                read_ranks(cluster, s.near + tid, ctas, o);
+#pragma unroll
+                for (int r = 0; r < kMaxCtas; ++r) t += o[r];
+                sums[tid] = t;
+            }
+            __syncthreads();
+            u64 before = sums[kNear], total = before + sums[kNear + 1];
+            for (int b = 0; b < kNear; ++b) total += sums[b];
+            const double want_d = ceil(static_cast<double>(share) * static_cast<double>(total));
+            u64 want = want_d > 1.0 ? static_cast<u64>(want_d) : 1ull;
+            if (want > total) want = total;
+            int bin = -1;
+            u64 need = 0;
+            if (want > before)
+                for (int b = 0; b < kNear && bin < 0; ++b) {
+                    if (want <= before + sums[b]) {
+                        bin = near_lo + b;
+                        need = want - before;
+                    }
+                    before += sums[b];
+                }
+            cluster.sync();                               // the sums are read
+            if (bin >= 0) {
+                cut_in_bin(bin, s.cum[bin] - (bin ? s.cum[bin - 1] : 0), false, 0, need);
+                settled = true;
+            } else {
+                near_lo = near_hi = -1;                   // somewhere else: all bins, below
+                kept_ahead = 0;
+            }
+        }
+        if (!settled) {
+            // exact weights of every bin of what is kept so far
+            Buckets b{reinterpret_cast<uint32_t*>(s.list), reinterpret_cast<uint32_t*>(s.list) + kBins};
+            b.clear();
             const int walk = sparse >= 0 ? sparse : p.slice;
             for (int j = tid; j < walk; j += kThreads) {
                 const float x = value(sparse >= 0 ? left[j] : j);
-                const uint32_t key = key_of(x);
-                if (k_on ? key <= cut_key : false) continue;
-                const int b = bin_of(x);
-                if (b >= kBins - 1) continue;
-                const u64 w = weight(x);
-                if (w == 0) continue;
-                const uint32_t wl = static_cast<uint32_t>(w);
-                const uint32_t old = atomicAdd(&lo[b], wl);
-                const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + wl < old);
-                if (up) atomicAdd(&hi[b], up);
+                // ties at a top-k cut: only cut_ties of them count, all of one weight and bin
+                if (k_on && key_of(x) <= cut_key) continue;
+                const int bin = bin_of(x);
+                const u64 w = bin < kBins - 1 ? weight(x) : 0;
+                if (w != 0) b.add(bin, w);
             }
             cluster.sync();
             u64 wb[4] = {0, 0, 0, 0};
+#pragma unroll 2
             for (int r = 0; r < ctas; ++r) {
-                const uint32_t* rl = cluster.map_shared_rank(lo, r);
+                const uint32_t* rl = cluster.map_shared_rank(b.lo, r);
                 const uint4 l = reinterpret_cast<const uint4*>(rl)[tid];
                 const uint4 h = reinterpret_cast<const uint4*>(rl + kBins)[tid];
-                wb[0] += static_cast<u64>(h.x) << 32 | 0; wb[0] += l.x;
-                wb[1] += static_cast<u64>(h.y) << 32 | 0; wb[1] += l.y;
-                wb[2] += static_cast<u64>(h.z) << 32 | 0; wb[2] += l.z;
-                wb[3] += static_cast<u64>(h.w) << 32 | 0; wb[3] += l.w;
+                wb[0] += (static_cast<u64>(h.x) << 32) + l.x;
+                wb[1] += (static_cast<u64>(h.y) << 32) + l.y;
+                wb[2] += (static_cast<u64>(h.z) << 32) + l.z;
+                wb[3] += (static_cast<u64>(h.w) << 32) + l.w;
             }
-            u64 tie_w = 0;
             if (k_on) {
-                tie_w = weight(value_of(cut_key));
-                const int b = bin_of(value_of(cut_key));
-                if (b >> 2 == tid && b < kBins - 1) {
+                const u64 tie_w = weight(value_of(cut_key));
+                const int bin = bin_of(value_of(cut_key));
+                if (bin >> 2 == tid && bin < kBins - 1) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if ((b & 3) == e) wb[e] += tie_w * cut_ties;
+                        if ((bin & 3) == e) wb[e] += tie_w * cut_ties;
                 }
             }
             u64 total;
             const u64 sum4 = wb[0] + wb[1] + wb[2] + wb[3];
             u64 before = block_inclusive(sum4, s.scan, &total) - sum4;
-            // the bins past the bound were not summed here
-            const u64 whole_w = have_all ? all : total;
-            const double want_d = ceil(static_cast<double>(share) * static_cast<double>(whole_w));
+            const double want_d = ceil(static_cast<double>(share) * static_cast<double>(total));
             u64 want = want_d > 1.0 ? static_cast<u64>(want_d) : 1ull;
             if (want > total) want = total;
 #pragma unroll
@@ -946,14 +1017,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const bool cut = cut_ties != 0xffffffffu;
     if (cut) {
         uint32_t ties = 0;
-        for (int j = lo; j < hi; ++j) ties += key_of(value(index(j))) == cut_key;
+        if (sparse >= 0) {
+            for (int j = lo; j < hi; ++j) ties += key_of(value(left[j])) == cut_key;
+        } else {
+            const float at = value_of(cut_key);           // (the same for both zeros)
+            for (int v = first_vec; v < last_vec; ++v) {
+                const uint4 q = xv[v];
+                const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) ties += to_float(e[k]) == at;
+            }
+        }
         uint32_t all;
         ties_before = block_inclusive(ties, s.scan32, &all) - ties;
         if (tid == 0) s.ties = all;
         cluster.sync();
         for (int r = 0; r < rank; ++r) ties_before += *cluster.map_shared_rank(&s.ties, r);
     }
-    u64 sum = 0;
+    u64 sum = kept_ahead;
     {
         uint32_t seen = ties_before;
         auto add = [&](float x) {
@@ -970,7 +1051,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 const uint4 q = xv[v];
                 const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) add(to_float(e[k]));
+                for (int k = 0; k < kVec; ++k) {
+                    const float x = to_float(e[k]);
+                    // the bins before the cut's neighbourhood are in kept_ahead already
+                    if (near_lo > 0 && bin_of(x) < near_lo) continue;
+                    add(x);
+                }
             }
         }
     }
