@@ -77,7 +77,7 @@ struct Shared {
     float scanf[kWarps];
     uint32_t ties;                          // this CTA's tokens at the cut
     uint32_t count;                         // a count exchanged between CTAs
-    uint32_t found;                         // a thread's find, for its CTA
+    uint32_t found, found2;                 // a thread's find, for its CTA
     uint32_t found_above;
     uint32_t list_n;                        // (leader) tokens in the list
     uint32_t cut_key;                       // (leader) the cut, for all CTAs
@@ -96,9 +96,9 @@ struct Weights {
     float topf;
     const double* pow2;
     __device__ __forceinline__ u64 operator()(float x) const {
-        if (x == topf) return 1ull << kFraction;
+        // no branches: the chains of several tokens overlap
         const double d = static_cast<double>(x) - top;
-        if (!(d * inv >= static_cast<double>(kCut))) return 0;
+        const bool counts = d * inv >= static_cast<double>(kCut);
         const double y = d * inv512;
         const double magic = 6755399441055744.0;                     // 1.5 * 2^52: rounds to integer
         const double shifted = y + magic;
@@ -111,7 +111,8 @@ struct Weights {
         const long long scale = static_cast<long long>((n >> 9) + kFraction) << 52;
         const double t = __longlong_as_double(__double_as_longlong(pow2[n & 511]) + scale);
         // t * e <= 2^44: adding 2^52 leaves the nearest integer in the low mantissa bits
-        return static_cast<u64>(__double_as_longlong(fma(t, e, 4503599627370496.0))) & 0xfffffffffffffull;
+        const u64 w = static_cast<u64>(__double_as_longlong(fma(t, e, 4503599627370496.0))) & 0xfffffffffffffull;
+        return x == topf ? 1ull << kFraction : counts ? w : 0ull;
     }
 };
 
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             const uint32_t before = block_inclusive(mine, s.scan32, &counted) - mine;
             reinterpret_cast<uint4*>(s.cum)[tid] =
                 make_uint4(before + c.x, before + c.x + c.y, before + c.x + c.y + c.z, before + mine);
-            if (tid == 0) s.found = kBins - 1;
+            if (tid == 0) s.found = s.found2 = kBins - 1;
             __syncthreads();
             return before;
         };
@@ -695,21 +696,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             const float w2 = w1 + c.z * low(4 * tid + 2), w3 = w2 + c.w * low(4 * tid + 3);
             float total;
             const float before = block_inclusive(w3, s.scanf, &total) - w3;
-            // the first bin at which the running sum reaches `want`
-            auto first = [&](float want) {
-                if (tid == 0) s.found = last - 1;
-                __syncthreads();
+            // the first bins at which the running sum reaches what is surely, and what is probably
+            // enough (tokens that were not counted weigh 1 - share at most); merge() has set
+            // found, the barriers of the prefix sum lie between
+            auto first = [&](float want, uint32_t* found) {
                 if (before + w3 >= want)
-                    atomicMin(&s.found, 4u * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
-                                                    : before + w2 >= want ? 2 : 3));
-                __syncthreads();
-                const int b = s.found;
-                __syncthreads();
-                return b;
+                    atomicMin(found, 4u * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
+                                                 : before + w2 >= want ? 2 : 3));
             };
-            // tokens that were not counted weigh 1 - share at most
-            p_bin = first(share * (total * kHigh + (1.0f - share)) * 1.0001f);
-            p_near = first(share * total);
+            first(share * (total * kHigh + (1.0f - share)) * 1.0001f, &s.found);
+            first(share * total, &s.found2);
+            __syncthreads();
+            p_bin = min(static_cast<int>(s.found), last - 1);
+            p_near = min(static_cast<int>(s.found2), last - 1);
         }
         const int bound = k_on ? (p_on ? k_bin : min(k_bin, m_bin)) : min(p_bin, m_bin);
         const uint32_t kept = s.cum[bound];
@@ -899,24 +898,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 for (int k = 0; k < kVec; ++k) {
                     const float x = to_float(e[k]);
                     const int b = bin_of(x);
-                    if (b >= kBins - 1) continue;
                     const u64 w = weight(x);
-                    if (b < near_lo) {
-                        ahead += w;
-                        kept_ahead += w >= least_w ? w : 0;
-                    } else if (b > near_hi) {
-                        behind += w;
-                    } else {
-                        Buckets{lo, lo + kNear}.add(b - near_lo, w);
-                    }
+                    ahead += b < near_lo ? w : 0;
+                    kept_ahead += b < near_lo && w >= least_w ? w : 0;
+                    behind += b > near_hi ? w : 0;
+                    if (b >= near_lo && b <= near_hi) Buckets{lo, lo + kNear}.add(b - near_lo, w);
                 }
             }
-            u64 mine;
-            block_inclusive(ahead, s.scan, &mine);
-            if (tid == 0) s.near[kNear] = mine;
-            block_inclusive(behind, s.scan, &mine);       // its barriers also end the bins' sums
-            if (tid == 0) s.near[kNear + 1] = mine;
+            ahead = warp_sum(ahead);
+            behind = warp_sum(behind);
+            if (lane == 0) {
+                s.warp_sum[warp] = ahead;
+                s.scan[warp] = behind;
+            }
+            __syncthreads();
             if (tid < kNear) s.near[tid] = (static_cast<u64>(lo[kNear + tid]) << 32) + lo[tid];
+            else if (tid < kNear + 2) {
+                u64 t = 0;
+                for (int w = 0; w < kWarps; ++w) t += tid == kNear ? s.warp_sum[w] : s.scan[w];
+                s.near[tid] = t;
+            }
             cluster.sync();
             u64* sums = s.list + kNear;                   // past the words above
             if (tid < kNear + 2) {
@@ -1032,30 +1033,43 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         ties_before = block_inclusive(ties, s.scan32, &all) - ties;
         if (tid == 0) s.ties = all;
         cluster.sync();
-        for (int r = 0; r < rank; ++r) ties_before += *cluster.map_shared_rank(&s.ties, r);
+        uint32_t o[kMaxCtas];
+        read_ranks(cluster, &s.ties, rank, o);
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) ties_before += o[r];
     }
     u64 sum = kept_ahead;
     {
         uint32_t seen = ties_before;
-        auto add = [&](float x) {
+        auto kept = [&](float x, u64 w) {
             const uint32_t key = key_of(x);
-            if (key < cut_key) return;
-            if (cut && key == cut_key && seen++ >= cut_ties) return;
-            const u64 w = weight(x);
-            sum += w >= least_w ? w : 0;
+            bool keep = key >= cut_key && w >= least_w;
+            if (cut && key == cut_key) keep = keep && seen++ < cut_ties;
+            return keep ? w : 0;
         };
         if (sparse >= 0) {
-            for (int j = lo; j < hi; ++j) add(value(left[j]));
+            for (int j = lo; j < hi; ++j) {
+                const float x = value(left[j]);
+                sum += kept(x, weight(x));
+            }
         } else {
             for (int v = first_vec; v < last_vec; ++v) {
                 const uint4 q = xv[v];
                 const T* e = reinterpret_cast<const T*>(&q);
+                if (near_lo > 0) {                        // few are left to weigh
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) {
-                    const float x = to_float(e[k]);
-                    // the bins before the cut's neighbourhood are in kept_ahead already
-                    if (near_lo > 0 && bin_of(x) < near_lo) continue;
-                    add(x);
+                    for (int k = 0; k < kVec; ++k) {
+                        // the bins before the cut's neighbourhood are in kept_ahead already
+                        const float x = to_float(e[k]);
+                        const int b = bin_of(x);
+                        if (b >= near_lo && b <= near_hi) sum += kept(x, weight(x));
+                    }
+                } else {
+                    u64 w[kVec];
+#pragma unroll
+                    for (int k = 0; k < kVec; ++k) w[k] = weight(to_float(e[k]));
+#pragma unroll
+                    for (int k = 0; k < kVec; ++k) sum += kept(to_float(e[k]), w[k]);
                 }
             }
         }
@@ -1065,10 +1079,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     if (tid == 0) s.sum = mine_total;
     cluster.sync();
     u64 total = 0, before = 0;
-    for (int r = 0; r < ctas; ++r) {
-        const u64 o = *cluster.map_shared_rank(&s.sum, r);
-        if (r < rank) before += o;
-        total += o;
+    {
+        u64 o[kMaxCtas];
+        read_ranks(cluster, &s.sum, ctas, o);
+#pragma unroll
+        for (int r = 0; r < kMaxCtas; ++r) {
+            if (r < rank) before += o[r];
+            total += o[r];
+        }
     }
     const u64 want = target_of(total);
     if (before <= want && want < before + mine_total) {   // the token is in this CTA
