@@ -11,8 +11,8 @@
 //
 // A thread-block cluster holds one row in the shared memory of its CTAs (the row is read from
 // HBM once) and agrees on maxima, counts and sums through distributed shared memory.  Nothing
-// is sorted as a whole: a histogram over 2047 bins of d (monotone in x) bounds the part of the
-// row that can be kept, from counts alone (a bin's weights differ by 1.5%, so the nucleus is
+// is sorted as a whole: a histogram over 1023 bins of d (monotone in x) bounds the part of the
+// row that can be kept, from counts alone (a bin's weights differ by 3%, so the nucleus is
 // bounded from above).  Where at most kList tokens are left, one CTA sorts those and settles
 // everything exactly; otherwise the cut is found bin by bin, from exact weights per bin, and
 // inside its bin by sorting it or, if ties make it large, by halving the range of values.
@@ -37,14 +37,17 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 8;                 // of a row's cluster
-constexpr int kBins = 2048;                 // the last one is not counted: weight 0
+constexpr int kBins = 1024;                 // the last one is not counted: weight 0
 constexpr int kList = 2048;
+constexpr int kCounted = 256;               // tokens that are compared all with all
+constexpr int kEach = kList / kThreads;     // listed tokens per thread
 constexpr int kByMaxima = 1024;             // largest top-k that is bounded by the threads' maxima
 constexpr int kNear = 5;                    // bins around where a top-p cut is expected
-constexpr int kSparse = 4096;               // listed tokens of a slice (16-bit places over the counts)
+constexpr int kSparse = 2048;               // listed tokens of a slice (16-bit places over the counts)
 constexpr float kCut = -30.0f;
 constexpr int kFraction = 44;
-static_assert(kThreads == 512, "one thread per entry of the table of powers");
+static_assert(kThreads == 512 && kBins == 2 * kThreads,
+              "one thread per entry of the table of powers, and per two bins");
 constexpr float kBinsPerNat = (kBins - 1) / 30.25f;
 typedef unsigned long long u64;
 
@@ -84,9 +87,12 @@ struct Shared {
     uint32_t cut_ties;
     u64 bin_above;
     u64 near[kNear + 2];                    // weights of the bins around a cut, before and behind
+    u64 near_all[kNear + 2];                // the same of the row
+    uint32_t warp_ties[kWarps];
     __align__(16) uint32_t hist[kBins];     // counts of this CTA
     __align__(16) uint32_t cum[kBins];      // counts of the row, inclusive prefix
-    __align__(16) u64 list[kList];          // (leader) tokens as (key, ~index); or per-bin weights
+    __align__(16) uint32_t work[2 * kList]; // sums by bucket; weights of listed tokens
+    __align__(16) u64 list[kList];          // (leader) tokens as ~(key, ~index)
 };
 
 // Weight of a token in units of 2^-44.  2^(y / 512) = 2^(n / 512) * exp(r): a table for the
@@ -154,47 +160,6 @@ __device__ __forceinline__ V block_inclusive(V v, V* scratch, V* total) {
     return v + base;
 }
 
-// Sorts n distinct words ascending by the CTA (the rest up to a power of two is ~0): each to
-// the place that the number of smaller ones gives, up to kCounted of them (measured at 60:
-// 0.5 us against 2), a bitonic sort above.
-constexpr int kCounted = 256;
-__device__ void sort_words(u64* a, int count, int n, uint32_t* scratch) {
-    if (n <= kCounted) {
-        // kThreads / n threads per word, each compares with its share of the words
-        const int per = kThreads / n, i = threadIdx.x / per, part = threadIdx.x % per;
-        __syncthreads();
-        const u64 x = a[i];
-        int below = 0;
-        if (i < count)
-            for (int k = part; k < count; k += per) below += a[k] < x;
-        for (int d = 1; d < per && d < 32; d <<= 1) below += __shfl_xor_sync(0xffffffffu, below, d);
-        if (per > 32) {
-            if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = below;
-            __syncthreads();
-            below = 0;
-            for (int w = 0; w < per / 32; ++w) below += scratch[i * (per / 32) + w];
-        }
-        __syncthreads();
-        if (part == 0 && i < count) a[below] = x;
-        __syncthreads();
-        return;
-    }
-    for (int k = 2; k <= n; k <<= 1)
-        for (int j = k >> 1; j; j >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-                const int lo = 2 * i - (i & (j - 1));
-                const int hi = lo + j;
-                const u64 x = a[lo], y = a[hi];
-                if ((x > y) == ((lo & k) == 0)) {
-                    a[lo] = y;
-                    a[hi] = x;
-                }
-            }
-        }
-    __syncthreads();
-}
-
 __device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
 
 // What a row asks of its list.
@@ -226,17 +191,16 @@ struct Buckets {
     // found, above: one shared word each, the bucket and the sum before it
     __device__ __forceinline__ void find(u64 want, u64* scratch, uint32_t* found, u64* above) {
         __syncthreads();
-        const uint4 l = reinterpret_cast<const uint4*>(lo)[threadIdx.x];
-        const uint4 h = reinterpret_cast<const uint4*>(hi)[threadIdx.x];
-        const u64 w[4] = {(static_cast<u64>(h.x) << 32) + l.x, (static_cast<u64>(h.y) << 32) + l.y,
-                          (static_cast<u64>(h.z) << 32) + l.z, (static_cast<u64>(h.w) << 32) + l.w};
+        const uint2 l = reinterpret_cast<const uint2*>(lo)[threadIdx.x];
+        const uint2 h = reinterpret_cast<const uint2*>(hi)[threadIdx.x];
+        const u64 w[2] = {(static_cast<u64>(h.x) << 32) + l.x, (static_cast<u64>(h.y) << 32) + l.y};
         u64 total;
-        const u64 mine = w[0] + w[1] + w[2] + w[3];
+        const u64 mine = w[0] + w[1];
         u64 before = block_inclusive(mine, scratch, &total) - mine;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2; ++e) {
             if (before <= want && want < before + w[e]) {
-                *found = 4 * threadIdx.x + e;
+                *found = 2 * threadIdx.x + e;
                 *above = before;
             }
             before += w[e];
@@ -245,19 +209,69 @@ struct Buckets {
     }
 };
 
-// Settles a row whose kept tokens are all among the `count` of s.list (any order, as
-// ~(key, ~index)), by one CTA.  `all`: weight of the whole row, 0: that of the list (its first
-// k).  Each cut is found by buckets (bins of d, then ranges of the index), exactly inside the
-// one bucket where it falls; up to kCounted tokens are compared all with all instead.
+// Threads that share a token when `count` tokens are compared all with all: within a warp, at
+// most a warp, and a divisor of the block.
+__device__ __forceinline__ int threads_per(int count) {
+    return count <= kThreads / 32 ? 32 : count <= kThreads ? kThreads / power_of_two(count) : 1;
+}
+
+// Of tokens ordered by (bucket, key), both ascending, the key at which the running sum of w
+// exceeds `want`.  Up to kEach tokens per thread; those with w == 0 are not there.  Sums by
+// bucket first, then all with all inside the one bucket.  Writes s.work and s.list.
+__device__ u64 locate(Shared& s, const int (&bucket)[kEach], const u64 (&key)[kEach], const u64 (&w)[kEach],
+                      u64 want) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    Buckets b{s.work, s.work + kBins};
+    __syncthreads();
+    b.clear();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (w[e] != 0) b.add(bucket[e], w[e]);
+    if (tid == 0) s.count = 0;
+    b.find(want, s.scan, &s.found, &s.bin_above);
+    const int at = s.found;
+    want -= s.bin_above;
+    u64* ws = reinterpret_cast<u64*>(s.work);             // the buckets are read
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (w[e] != 0 && bucket[e] == at) {
+            const uint32_t i = atomicAdd(&s.count, 1u);
+            s.list[i] = key[e];
+            ws[i] = w[e];
+        }
+    __syncthreads();
+    const int n = s.count, per = threads_per(n);
+    const unsigned group = per == 32 ? 0xffffffffu : ((1u << per) - 1) << (lane / per * per);
+    for (int i = tid / per; i < n; i += kThreads / per) {
+        const u64 k = s.list[i];
+        u64 before = 0;
+        for (int j = tid % per; j < n; j += per)
+            if (s.list[j] < k) before += ws[j];
+        for (int d = 1; d < per; d <<= 1) before += __shfl_xor_sync(group, before, d);
+        if (before <= want && want < before + ws[i]) s.best = k;
+    }
+    __syncthreads();
+    return s.best;
+}
+
+__device__ __forceinline__ u64 sum_of(Shared& s, const u64 (&w)[kEach]) {
+    u64 mine = 0, total;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) mine += w[e];
+    block_inclusive(mine, s.scan, &total);
+    return total;
+}
+
+// Settles a row whose kept tokens are all among the `count` of s.list (any order), by one CTA.
+// `all`: weight of the whole row, 0: that of the list (its first k).
 template <class W, class B, class G>
 __device__ void settle_list(Shared& s, int count, const ListRow& r, const W& weight, const B& bin_of,
                             const G& target_of, u64 all) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (count <= kCounted) {
-        // kThreads / m threads per token, at most a warp
-        const int m = power_of_two(count), per = min(32, kThreads / m), i = tid / per, part = tid % per;
-        u64* ws = reinterpret_cast<u64*>(s.cum);          // weights by rank, then the kept ones
-        int* at = reinterpret_cast<int*>(s.cum + 2 * kCounted);
+        const int per = threads_per(count), i = tid / per, part = tid % per;
+        u64* ws = reinterpret_cast<u64*>(s.work);         // weights by rank, then the kept ones
+        int* at = reinterpret_cast<int*>(s.work + 2 * kCounted);
         const u64 x = i < count ? s.list[i] : 0;
         int ahead = 0;
         if (i < count)
@@ -270,11 +284,11 @@ __device__ void settle_list(Shared& s, int count, const ListRow& r, const W& wei
         }
         __syncthreads();
         if (warp == 0) {
-            constexpr int kEach = kCounted / 32;
-            u64 w[kEach], mine = 0;
+            constexpr int kMine = kCounted / 32;
+            u64 w[kMine], mine = 0;
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int j = lane * kEach + e;
+            for (int e = 0; e < kMine; ++e) {
+                const int j = lane * kMine + e;
                 w[e] = j < count && (r.k == 0 || j < r.k) ? ws[j] : 0;
                 mine += w[e];
             }
@@ -289,8 +303,8 @@ __device__ void settle_list(Shared& s, int count, const ListRow& r, const W& wei
             const double want = static_cast<double>(r.share) * static_cast<double>(all ? all : total);
             mine = 0;
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int j = lane * kEach + e;
+            for (int e = 0; e < kMine; ++e) {
+                const int j = lane * kMine + e;
                 const bool keep = w[e] >= r.least_w && (!r.p_on || j == 0 || static_cast<double>(before) < want);
                 before += w[e];
                 if (!keep) w[e] = 0;
@@ -310,114 +324,48 @@ __device__ void settle_list(Shared& s, int count, const ListRow& r, const W& wei
         return;
     }
 
-    constexpr int kEach = kList / kThreads;
     u64 x[kEach], w[kEach];
-    int bin[kEach];
+    int bucket[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const int i = tid + e * kThreads;
         x[e] = i < count ? s.list[i] : ~0ull;
         const float v = value_of(static_cast<uint32_t>(~x[e] >> 32));
-        bin[e] = i < count ? bin_of(v) : kBins;
+        bucket[e] = i < count ? bin_of(v) : 0;
         w[e] = i < count ? weight(v) : 0;
     }
-    __syncthreads();
-    Buckets b{s.hist, s.cum};
-    // Tokens of a bucket, by a key to sort by (ascending), in the list's place, their weights in
-    // the buckets'; returns how many.
-    u64* const ws = reinterpret_cast<u64*>(s.hist);
-    auto collect = [&](int bucket, const int (&of)[kEach], const u64 (&key)[kEach]) {
-        if (tid == 0) s.count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-            if (of[e] == bucket && w[e] != 0) {
-                const uint32_t at = atomicAdd(&s.count, 1u);
-                s.list[at] = key[e];
-                ws[at] = w[e];
-            }
-        __syncthreads();
-        return static_cast<int>(s.count);
-    };
-    // The key in a collected bucket at which the running sum of `unit ? 1 : weight` exceeds `want`.
-    auto settle = [&](int n, u64 want, bool unit) {
-        const int per = n <= 16 ? 32 : n <= kCounted ? kThreads / power_of_two(n) : 1;
-        for (int i = tid / per; i < n; i += kThreads / per) {
-            // every thread of a group runs the same rounds; groups lie within a warp
-            const u64 key = s.list[i], mine = unit ? 1 : ws[i];
-            u64 before = 0;
-            for (int j = tid % per; j < n; j += per)
-                if (s.list[j] < key) before += unit ? 1 : ws[j];
-            const unsigned group = per == 32 ? 0xffffffffu : ((1u << per) - 1) << (lane / per * per);
-            for (int d = 1; d < per; d <<= 1) before += __shfl_xor_sync(group, before, d);
-            if (before <= want && want < before + mine) s.best = key;
-        }
-        __syncthreads();
-        return s.best;
-    };
-    auto sum_of = [&]() {
-        u64 mine = 0, total;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) mine += w[e];
-        block_inclusive(mine, s.scan, &total);
-        return total;
-    };
     if (r.k > 0) {
-        int some = 0, all_some;                           // tokens that weigh something
+        u64 one[kEach];                                   // tokens that weigh something
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) some += w[e] != 0;
-        block_inclusive(some, reinterpret_cast<int*>(s.scan32), &all_some);
-        if (r.k < all_some) {
-            b.clear();
-#pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                if (w[e] != 0) atomicAdd(&b.lo[bin[e]], 1u);
-            b.find(r.k - 1, s.scan, &s.found, &s.bin_above);
-            const u64 above = s.bin_above;
-            const int n = collect(s.found, bin, x);
-            const u64 cut = settle(n, r.k - 1 - above, true);
+        for (int e = 0; e < kEach; ++e) one[e] = w[e] != 0;
+        if (static_cast<u64>(r.k) < sum_of(s, one)) {
+            const u64 cut = locate(s, bucket, x, one, r.k - 1);
 #pragma unroll
             for (int e = 0; e < kEach; ++e)
                 if (x[e] > cut) w[e] = 0;
         }
     }
     if (r.p_on) {
-        const u64 total = sum_of();
+        const u64 total = sum_of(s, w);
         // kept while the sum before a token is below share * total: up to the first token at
         // which the running sum exceeds the last whole number below that
         const double want_d = ceil(static_cast<double>(r.share) * static_cast<double>(all ? all : total)) - 1.0;
         u64 want = want_d > 0.0 ? static_cast<u64>(want_d) : 0ull;
         if (want > total - 1) want = total - 1;
-        b.clear();
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-            if (w[e] != 0) b.add(bin[e], w[e]);
-        b.find(want, s.scan, &s.found, &s.bin_above);
-        const u64 above = s.bin_above;
-        const int n = collect(s.found, bin, x);
-        const u64 cut = settle(n, want - above, false);
+        const u64 cut = locate(s, bucket, x, w, want);
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
             if (x[e] > cut) w[e] = 0;
     }
-    u64 index[kEach];
-    int range[kEach];
-    const int shift = max(0, 32 - __clz(r.V - 1) - 11);   // 2048 ranges of indices
+    const int shift = max(0, 32 - __clz(r.V - 1) - 10);   // 1024 ranges of indices
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         if (w[e] < r.least_w) w[e] = 0;
-        index[e] = 0xffffffffu - static_cast<uint32_t>(~x[e]);
-        range[e] = w[e] != 0 ? static_cast<int>(index[e] >> shift) : kBins;
+        x[e] = 0xffffffffu - static_cast<uint32_t>(~x[e]);
+        bucket[e] = static_cast<int>(x[e] >> shift) & (kBins - 1);
     }
-    const u64 want = target_of(sum_of());
-    b.clear();
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-        if (w[e] != 0) b.add(range[e], w[e]);
-    b.find(want, s.scan, &s.found, &s.bin_above);
-    const u64 above = s.bin_above;
-    const int n = collect(s.found, range, index);
-    const u64 token = settle(n, want - above, false);
+    const u64 want = target_of(sum_of(s, w));
+    const u64 token = locate(s, bucket, x, w, want);
     if (tid == 0) *r.token = static_cast<int64_t>(token);
 }
 
@@ -547,15 +495,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         return t >= static_cast<double>(most) ? most : t > 0.0 ? static_cast<u64>(t) : 0ull;
     };
 
-    // A thread's part of the slice in index order: an odd number of vectors, so that the 16-byte
-    // reads of eight neighbours fall on different banks.
-    const int part_vecs = ((vecs + kThreads - 1) / kThreads) | 1;
-    const int first_vec = min(tid * part_vecs, vecs), last_vec = min(first_vec + part_vecs, vecs);
+    // In index order a warp has a contiguous part of the slice, 32 vectors at a time.
+    const int part_vecs = (vecs + kWarps - 1) / kWarps;
+    const int first_vec = min(warp * part_vecs, vecs), last_vec = min(first_vec + part_vecs, vecs);
     // tokens of the slice that can be kept, by index (over the counts); -1: not listed
     uint16_t* const left = reinterpret_cast<uint16_t*>(s.hist);
     int sparse = -1;
     // bins around a top-p cut, and this part's kept weight in those before them
-    int near_lo = -1, near_hi = -1;
+    int near_lo = -1, near_hi = -2;
     u64 kept_ahead = 0;
 
     // ---- the cut: kept are keys above cut_key and the first cut_ties (by index) at it
@@ -607,34 +554,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         };
         // counts of the row by bin, from those of the CTAs: an inclusive prefix in s.cum, the
         // thread's four bins in c, its prefix before them returned
-        uint4 c;
+        uint2 c;
         uint32_t counted;
         auto merge = [&]() {
-            uint4 o[kMaxCtas];
+            uint2 o[kMaxCtas];
 #pragma unroll
             for (int r = 0; r < kMaxCtas; ++r)
-                o[r] = r < ctas ? reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.hist, r))[tid]
-                                : make_uint4(0, 0, 0, 0);
+                o[r] = r < ctas ? reinterpret_cast<const uint2*>(cluster.map_shared_rank(s.hist, r))[tid]
+                                : make_uint2(0, 0);
             c = o[0];
 #pragma unroll
             for (int r = 1; r < kMaxCtas; ++r) {
-                c.x += o[r].x; c.y += o[r].y; c.z += o[r].z; c.w += o[r].w;
+                c.x += o[r].x;
+                c.y += o[r].y;
             }
-            const uint32_t mine = c.x + c.y + c.z + c.w;
-            const uint32_t before = block_inclusive(mine, s.scan32, &counted) - mine;
-            reinterpret_cast<uint4*>(s.cum)[tid] =
-                make_uint4(before + c.x, before + c.x + c.y, before + c.x + c.y + c.z, before + mine);
             if (tid == 0) s.found = s.found2 = kBins - 1;
-            __syncthreads();
+            const uint32_t mine = c.x + c.y;
+            const uint32_t before = block_inclusive(mine, s.scan32, &counted) - mine;
+            reinterpret_cast<uint2*>(s.cum)[tid] = make_uint2(before + c.x, before + mine);
             return before;
         };
-        // the bin in which the count-th token lies (all bins: not among the counted)
+        // the bin in which the count-th token lies (the last: not among the counted); a barrier
         auto bin_of_count = [&](uint32_t before, uint32_t count) {
-            if (before < count && count <= before + c.x + c.y + c.z + c.w) {
-                count -= before;
-                s.found = 4 * tid + (count <= c.x ? 0 : count <= c.x + c.y ? 1
-                                     : count <= c.x + c.y + c.z ? 2 : 3);
-            }
+            if (before < count && count <= before + c.x + c.y)
+                s.found = 2 * tid + (count <= before + c.x ? 0 : 1);
             __syncthreads();
             return static_cast<int>(s.found);
         };
@@ -686,23 +629,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         // tokens past the counted bins weigh nothing, so a top-k that reaches them cuts nothing
         k_on = k_on && static_cast<uint32_t>(k) <= counted;
         const int k_bin = k_on ? bin_of_count(before_bins, k) : kBins - 1;
-        // Top-p without top-k: the bins' weights lie within 1.5% (a thousandth for rounding), so
+        // Top-p without top-k: the bins' weights lie within 3% (a thousandth for rounding), so
         // the cut is surely not past p_bin, and probably within two bins of p_near.
         int p_bin = last - 1, p_near = 0;
         if (p_on && !k_on) {
             auto low = [](int b) { return exp2f((b + 1) * (-1.44269504f / kBinsPerNat)) * 0.999f; };
-            constexpr float kHigh = 1.018f;               // top of a bin over its low
-            const float w0 = c.x * low(4 * tid), w1 = w0 + c.y * low(4 * tid + 1);
-            const float w2 = w1 + c.z * low(4 * tid + 2), w3 = w2 + c.w * low(4 * tid + 3);
+            constexpr float kHigh = 1.033f;               // top of a bin over its low
+            const float w0 = c.x * low(2 * tid), w1 = w0 + c.y * low(2 * tid + 1);
             float total;
-            const float before = block_inclusive(w3, s.scanf, &total) - w3;
+            const float before = block_inclusive(w1, s.scanf, &total) - w1;
             // the first bins at which the running sum reaches what is surely, and what is probably
-            // enough (tokens that were not counted weigh 1 - share at most); merge() has set
-            // found, the barriers of the prefix sum lie between
+            // enough (tokens that were not counted weigh 1 - share at most)
             auto first = [&](float want, uint32_t* found) {
-                if (before + w3 >= want)
-                    atomicMin(found, 4u * tid + (before + w0 >= want ? 0 : before + w1 >= want ? 1
-                                                 : before + w2 >= want ? 2 : 3));
+                const bool reached = before + w1 >= want;
+                const unsigned m = __ballot_sync(0xffffffffu, reached);
+                if (reached && lane == __ffs(m) - 1) atomicMin(found, 2u * tid + (before + w0 >= want ? 0 : 1));
             };
             first(share * (total * kHigh + (1.0f - share)) * 1.0001f, &s.found);
             first(share * total, &s.found2);
@@ -710,6 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             p_bin = min(static_cast<int>(s.found), last - 1);
             p_near = min(static_cast<int>(s.found2), last - 1);
         }
+        __syncthreads();                                  // s.cum
         const int bound = k_on ? (p_on ? k_bin : min(k_bin, m_bin)) : min(p_bin, m_bin);
         const uint32_t kept = s.cum[bound];
         if (kept <= kList) {
@@ -745,32 +687,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
 
         // ---- more than that is left: list this CTA's share by index, if it is few
-        cluster.sync();                                   // every CTA has read the counts
         if (k_on || !p_on) {
-            uint32_t mine_n = 0;
-            for (int v = first_vec; v < last_vec; ++v) {
-                const uint4 q = xv[v];
-                const T* e = reinterpret_cast<const T*>(&q);
+            cluster.sync();                               // every CTA has read the counts
+            auto hits_of = [&](int v) {                   // tokens of a vector that are left
+                unsigned hits = 0;
+                if (v < last_vec) {
+                    const uint4 q = xv[v];
+                    const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) {
-                    const int b = bin_of(to_float(e[k]));
-                    mine_n += b <= bound && b < kBins - 1;
+                    for (int k = 0; k < kVec; ++k) {
+                        const int b = bin_of(to_float(e[k]));
+                        if (b <= bound && b < kBins - 1) hits |= 1u << k;
+                    }
                 }
+                return hits;
+            };
+            uint32_t mine_n = 0;
+            for (int v = first_vec + lane; v < last_vec; v += 32) mine_n += __popc(hits_of(v));
+            mine_n = warp_sum(mine_n);
+            if (lane == 0) s.scan32[warp] = mine_n;
+            __syncthreads();
+            uint32_t at = 0, all_n = 0;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) at += s.scan32[w];
+                all_n += s.scan32[w];
             }
-            uint32_t all_n;
-            uint32_t at = block_inclusive(mine_n, s.scan32, &all_n) - mine_n;
             if (all_n <= kSparse && p.slice <= 65536) {
                 sparse = all_n;
-                if (mine_n)
-                    for (int v = first_vec; v < last_vec; ++v) {
-                        const uint4 q = xv[v];
-                        const T* e = reinterpret_cast<const T*>(&q);
+                for (int v0 = first_vec; v0 < last_vec; v0 += 32) {
+                    unsigned hits = hits_of(v0 + lane);
+                    uint32_t inc = __popc(hits);
 #pragma unroll
-                        for (int k = 0; k < kVec; ++k) {
-                            const int b = bin_of(to_float(e[k]));
-                            if (b <= bound && b < kBins - 1) left[at++] = v * kVec + k;
-                        }
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const uint32_t o = __shfl_up_sync(0xffffffffu, inc, d);
+                        if (lane >= d) inc += o;
                     }
+                    uint32_t to = at + inc - __popc(hits);
+                    for (; hits; hits &= hits - 1) left[to++] = (v0 + lane) * kVec + __ffs(hits) - 1;
+                    at += __shfl_sync(0xffffffffu, inc, 31);
+                }
             }
             __syncthreads();
         }
@@ -801,51 +756,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 gather(bin, bin);
                 cluster.sync();
                 if (rank == 0) {
-                    const int m2 = power_of_two(size);
-                    for (int i = size + tid; i < m2; i += kThreads) s.list[i] = ~0ull;
-                    sort_words(s.list, size, m2, s.scan32);
-                    constexpr int kEach = kList / kThreads;
-                    u64 w[kEach], mine_w = 0;
+                    // buckets: a 1024th of the bin each
+                    u64 x[kEach], w[kEach];
+                    int sub[kEach];
+                    const u64 goal = by_count ? count : need;
 #pragma unroll
                     for (int e = 0; e < kEach; ++e) {
-                        const int i = tid * kEach + e;
-                        const uint32_t key = static_cast<uint32_t>(~s.list[i] >> 32);
-                        w[e] = i < size && (key > cut_key || key == cut_key) ? weight(value_of(key)) : 0;
-                        mine_w += w[e];
+                        const int i = tid + e * kThreads;
+                        x[e] = i < size ? s.list[i] : ~0ull;
+                        const uint32_t key = static_cast<uint32_t>(~x[e] >> 32);
+                        const float v = value_of(key);
+                        w[e] = i >= size ? 0 : by_count ? 1 : key >= cut_key ? weight(v) : 0;
+                        const float z = v == top ? 0.0f : (top - v) * invf * kBinsPerNat - static_cast<float>(bin);
+                        sub[e] = min(max(static_cast<int>(z * kBins), 0), kBins - 1);
                     }
-                    u64 total;
-                    u64 before = block_inclusive(mine_w, s.scan, &total) - mine_w;
-                    if (tid == 0) s.found = size - 1;
-                    __syncthreads();
+                    const u64 last_kept = locate(s, sub, x, w, goal - 1);
+                    u64 same[kEach];
 #pragma unroll
-                    for (int e = 0; e < kEach; ++e) {
-                        const int i = tid * kEach + e;
-                        // last token kept: the count-th, or the first that reaches `need`
-                        if (i < size && (by_count ? i + 1u == count : before < need && before + w[e] >= need))
-                            s.found = i;
-                        before += w[e];
-                    }
-                    __syncthreads();
-                    const int last = s.found;
-                    const uint32_t key = static_cast<uint32_t>(~s.list[last] >> 32);
-                    uint32_t ties = 0;
-                    for (int i = tid; i <= last; i += kThreads)
-                        ties += static_cast<uint32_t>(~s.list[i] >> 32) == key;
-                    ties = warp_sum(ties);
-                    if (lane == 0) s.scan32[warp] = ties;
-                    __syncthreads();
+                    for (int e = 0; e < kEach; ++e) same[e] = x[e] <= last_kept && (x[e] ^ last_kept) >> 32 == 0;
+                    const u64 ties = sum_of(s, same);
                     if (tid == 0) {
-                        ties = 0;
-                        for (int i = 0; i < kWarps; ++i) ties += s.scan32[i];
-                        s.cut_key = key;
-                        s.cut_ties = ties;
-                        s.list_n = 0;
+                        s.cut_key = static_cast<uint32_t>(~last_kept >> 32);
+                        s.cut_ties = static_cast<uint32_t>(ties);
                     }
+                    if (tid == 0) s.list_n = 0;
                 }
                 cluster.sync();
                 cut_key = leader->cut_key;
                 cut_ties = leader->cut_ties;
-                cluster.sync();
                 return;
             }
             // largest key t with enough tokens (weight) at or above it, bit by bit
@@ -887,11 +825,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             // of the bins before the cut's neighbourhood, of each bin in it and of those behind.
             near_lo = max(p_near - 2, 0);
             near_hi = min(p_near + 2, last - 1);
-            uint32_t* lo = reinterpret_cast<uint32_t*>(s.list);
+            uint32_t* lo = s.work;
             if (tid < 2 * kNear) lo[tid] = 0;
             __syncthreads();
             u64 ahead = 0, behind = 0;
-            for (int v = first_vec; v < last_vec; ++v) {
+            for (int v = first_vec + lane; v < last_vec; v += 32) {
                 const uint4 q = xv[v];
                 const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
@@ -919,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 s.near[tid] = t;
             }
             cluster.sync();
-            u64* sums = s.list + kNear;                   // past the words above
+            u64* sums = s.near_all;
             if (tid < kNear + 2) {
                 u64 o[kMaxCtas], t = 0;
                 read_ranks(cluster, s.near + tid, ctas, o);
@@ -943,18 +881,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                     }
                     before += sums[b];
                 }
-            cluster.sync();                               // the sums are read
             if (bin >= 0) {
                 cut_in_bin(bin, s.cum[bin] - (bin ? s.cum[bin - 1] : 0), false, 0, need);
                 settled = true;
             } else {
-                near_lo = near_hi = -1;                   // somewhere else: all bins, below
+                near_lo = -1, near_hi = -2;                // somewhere else: all bins, below
                 kept_ahead = 0;
+                cluster.sync();
             }
         }
         if (!settled) {
             // exact weights of every bin of what is kept so far
-            Buckets b{reinterpret_cast<uint32_t*>(s.list), reinterpret_cast<uint32_t*>(s.list) + kBins};
+            Buckets b{s.work, s.work + kBins};
             b.clear();
             const int walk = sparse >= 0 ? sparse : p.slice;
             for (int j = tid; j < walk; j += kThreads) {
@@ -966,36 +904,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 if (w != 0) b.add(bin, w);
             }
             cluster.sync();
-            u64 wb[4] = {0, 0, 0, 0};
-#pragma unroll 2
+            u64 wb[2] = {0, 0};
+#pragma unroll 4
             for (int r = 0; r < ctas; ++r) {
                 const uint32_t* rl = cluster.map_shared_rank(b.lo, r);
-                const uint4 l = reinterpret_cast<const uint4*>(rl)[tid];
-                const uint4 h = reinterpret_cast<const uint4*>(rl + kBins)[tid];
+                const uint2 l = reinterpret_cast<const uint2*>(rl)[tid];
+                const uint2 h = reinterpret_cast<const uint2*>(rl + kBins)[tid];
                 wb[0] += (static_cast<u64>(h.x) << 32) + l.x;
                 wb[1] += (static_cast<u64>(h.y) << 32) + l.y;
-                wb[2] += (static_cast<u64>(h.z) << 32) + l.z;
-                wb[3] += (static_cast<u64>(h.w) << 32) + l.w;
             }
             if (k_on) {
                 const u64 tie_w = weight(value_of(cut_key));
                 const int bin = bin_of(value_of(cut_key));
-                if (bin >> 2 == tid && bin < kBins - 1) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if ((bin & 3) == e) wb[e] += tie_w * cut_ties;
-                }
+                if (bin >> 1 == tid && bin < kBins - 1) (bin & 1 ? wb[1] : wb[0]) += tie_w * cut_ties;
             }
             u64 total;
-            const u64 sum4 = wb[0] + wb[1] + wb[2] + wb[3];
-            u64 before = block_inclusive(sum4, s.scan, &total) - sum4;
+            u64 before = block_inclusive(wb[0] + wb[1], s.scan, &total) - wb[0] - wb[1];
             const double want_d = ceil(static_cast<double>(share) * static_cast<double>(total));
             u64 want = want_d > 1.0 ? static_cast<u64>(want_d) : 1ull;
             if (want > total) want = total;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
                 if (before < want && before + wb[e] >= want) {
-                    s.found = 4 * tid + e;
+                    s.found = 2 * tid + e;
                     s.bin_above = before;
                 }
                 before += wb[e];
@@ -1008,120 +939,125 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         }
     }
 
-    // ---- cumulative weights in index order: each thread a contiguous part of the slice, or of
-    // what is listed of it
-    const int each = sparse >= 0 ? (sparse + kThreads - 1) / kThreads : part_vecs * kVec;
-    const int walk = sparse >= 0 ? sparse : p.slice;
-    const int lo = min(tid * each, walk), hi = min(lo + each, walk);
-    auto index = [&](int j) { return sparse >= 0 ? static_cast<int>(left[j]) : j; };
-    uint32_t ties_before = 0;                             // at the cut, before this thread's part
+    // ---- cumulative weights in index order.  Tokens at the cut (of one weight) are counted
+    // apart, so that one exchange tells both how many of them a CTA keeps and what it holds.
     const bool cut = cut_ties != 0xffffffffu;
-    if (cut) {
-        uint32_t ties = 0;
-        if (sparse >= 0) {
-            for (int j = lo; j < hi; ++j) ties += key_of(value(left[j])) == cut_key;
-        } else {
-            const float at = value_of(cut_key);           // (the same for both zeros)
-            for (int v = first_vec; v < last_vec; ++v) {
-                const uint4 q = xv[v];
-                const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) ties += to_float(e[k]) == at;
-            }
-        }
-        uint32_t all;
-        ties_before = block_inclusive(ties, s.scan32, &all) - ties;
-        if (tid == 0) s.ties = all;
-        cluster.sync();
-        uint32_t o[kMaxCtas];
-        read_ranks(cluster, &s.ties, rank, o);
-#pragma unroll
-        for (int r = 0; r < kMaxCtas; ++r) ties_before += o[r];
-    }
+    u64 tie_w = cut ? weight(value_of(cut_key)) : 0;
+    if (tie_w < least_w) tie_w = 0;
+    auto kept = [&](float x, u64 w, int& ties) {
+        const uint32_t key = key_of(x);
+        const bool tie = cut && key == cut_key;
+        ties += tie;
+        return key >= cut_key && w >= least_w && !tie ? w : 0ull;
+    };
+    // a warp's part: vectors of the slice, or listed tokens
+    const int part = (sparse + kWarps - 1) / kWarps;
+    const int from = sparse >= 0 ? min(warp * part, sparse) : first_vec;
+    const int to = sparse >= 0 ? min(from + part, sparse) : last_vec;
     u64 sum = kept_ahead;
-    {
-        uint32_t seen = ties_before;
-        auto kept = [&](float x, u64 w) {
-            const uint32_t key = key_of(x);
-            bool keep = key >= cut_key && w >= least_w;
-            if (cut && key == cut_key) keep = keep && seen++ < cut_ties;
-            return keep ? w : 0;
-        };
+    int ties = 0;
+    auto weigh = [&](int v, u64& sum, int& ties) {        // a vector, or a listed token
         if (sparse >= 0) {
-            for (int j = lo; j < hi; ++j) {
-                const float x = value(left[j]);
-                sum += kept(x, weight(x));
-            }
+            const float x = value(left[v]);
+            sum += kept(x, weight(x), ties);
         } else {
-            for (int v = first_vec; v < last_vec; ++v) {
-                const uint4 q = xv[v];
-                const T* e = reinterpret_cast<const T*>(&q);
-                if (near_lo > 0) {                        // few are left to weigh
+            const uint4 q = xv[v];
+            const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
-                    for (int k = 0; k < kVec; ++k) {
-                        // the bins before the cut's neighbourhood are in kept_ahead already
-                        const float x = to_float(e[k]);
-                        const int b = bin_of(x);
-                        if (b >= near_lo && b <= near_hi) sum += kept(x, weight(x));
-                    }
-                } else {
-                    u64 w[kVec];
+            for (int k = 0; k < kVec; ++k) sum += kept(to_float(e[k]), weight(to_float(e[k])), ties);
+        }
+    };
+    for (int v = from + lane; v < to; v += 32) {
+        if (near_lo < 0) {
+            weigh(v, sum, ties);
+        } else {                                          // few are left to weigh
+            const uint4 q = xv[v];
+            const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
-                    for (int k = 0; k < kVec; ++k) w[k] = weight(to_float(e[k]));
-#pragma unroll
-                    for (int k = 0; k < kVec; ++k) sum += kept(to_float(e[k]), w[k]);
-                }
+            for (int k = 0; k < kVec; ++k) {
+                const float x = to_float(e[k]);
+                const int b = bin_of(x);
+                if (b >= near_lo && b <= near_hi) sum += kept(x, weight(x), ties);
             }
         }
     }
-    u64 mine_total;
-    const u64 inclusive = block_inclusive(sum, s.scan, &mine_total);
-    if (tid == 0) s.sum = mine_total;
+    sum = warp_sum(sum);
+    ties = warp_sum(ties);
+    if (lane == 0) {
+        s.warp_sum[warp] = sum;
+        s.warp_ties[warp] = ties;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        sum = 0;
+        ties = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            sum += s.warp_sum[w];
+            ties += s.warp_ties[w];
+        }
+        s.sum = sum;
+        s.ties = ties;
+    }
     cluster.sync();
-    u64 total = 0, before = 0;
+    // kept weight of what comes before a place with `sum` of weights and `ties` at the cut
+    auto with_ties = [&](u64 sum, u64 ties) { return sum + (ties < cut_ties ? ties : cut_ties) * tie_w; };
+    u64 before = 0, ties_before = 0, total;
     {
-        u64 o[kMaxCtas];
+        u64 o[kMaxCtas], all_sum = 0, all_ties = 0;
+        uint32_t o_ties[kMaxCtas];
         read_ranks(cluster, &s.sum, ctas, o);
+        read_ranks(cluster, &s.ties, ctas, o_ties);
 #pragma unroll
         for (int r = 0; r < kMaxCtas; ++r) {
-            if (r < rank) before += o[r];
-            total += o[r];
+            if (r < rank) {
+                before += o[r];
+                ties_before += o_ties[r];
+            }
+            all_sum += o[r];
+            all_ties += o_ties[r];
         }
+        total = with_ties(all_sum, all_ties);
     }
     const u64 want = target_of(total);
-    if (before <= want && want < before + mine_total) {   // the token is in this CTA
-        const u64 upto = before + inclusive;
-        if (upto - sum <= want && want < upto) {          // in this thread's part
-            s.found = lo;
-            s.found_above = ties_before;
-            s.bin_above = upto - sum;
-        }
-        __syncthreads();
-        if (warp == 0) {                                  // 32 tokens of the part at a time
-            const int from = s.found, to = min(from + each, walk);
-            uint32_t seen = s.found_above;
-            u64 at = s.bin_above;
-            for (int j0 = from; j0 < to && at <= want; j0 += 32) {
-                const int j = j0 + lane;
-                const float x = j < to ? value(index(j)) : __int_as_float(0xff800000);
-                const uint32_t key = key_of(x);
-                bool keep = j < to && key >= cut_key;
-                if (cut) {
-                    const unsigned m = __ballot_sync(0xffffffffu, keep && key == cut_key);
-                    if (keep && key == cut_key) keep = seen + __popc(m & ((1u << lane) - 1)) < cut_ties;
-                    seen += __popc(m);
-                }
-                u64 w = keep ? weight(x) : 0;
-                if (w < least_w) w = 0;
-                u64 inc = w;
+    for (int w = 0; w < warp; ++w) {
+        before += s.warp_sum[w];
+        ties_before += s.warp_ties[w];
+    }
+    if (with_ties(before, ties_before) <= want &&
+        want < with_ties(before + s.warp_sum[warp], ties_before + s.warp_ties[warp])) {
+        // the token is in this warp's part: 32 vectors (listed tokens) at a time
+        for (int v0 = from; v0 < to; v0 += 32) {
+            const int v = v0 + lane;
+            u64 mine = 0;
+            int mine_ties = 0;
+            if (v < to) weigh(v, mine, mine_ties);
+            u64 inc = mine;
+            int inc_ties = mine_ties;
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const u64 o = __shfl_up_sync(0xffffffffu, inc, d);
-                    if (lane >= d) inc += o;
+            for (int d = 1; d < 32; d <<= 1) {
+                const u64 o = __shfl_up_sync(0xffffffffu, inc, d);
+                const int t = __shfl_up_sync(0xffffffffu, inc_ties, d);
+                if (lane >= d) {
+                    inc += o;
+                    inc_ties += t;
                 }
-                if (at + inc - w <= want && want < at + inc) p.tokens[row] = base + index(j);
-                at += __shfl_sync(0xffffffffu, inc, 31);
             }
+            u64 at = before + inc - mine, at_ties = ties_before + inc_ties - mine_ties;
+            if (with_ties(at, at_ties) <= want && want < with_ties(before + inc, ties_before + inc_ties)) {
+                int i = sparse >= 0 ? static_cast<int>(left[v]) : v * kVec;
+                if (sparse < 0)
+                    for (;; ++i) {                        // one of the vector's tokens
+                        int tie = 0;
+                        const float x = value(i);
+                        at += kept(x, weight(x), tie);
+                        at_ties += tie;
+                        if (want < with_ties(at, at_ties) || i + 1 == (v + 1) * kVec) break;
+                    }
+                p.tokens[row] = base + i;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
+            ties_before += __shfl_sync(0xffffffffu, inc_ties, 31);
+            if (with_ties(before, ties_before) > want) break;
         }
     }
     cluster.sync();
