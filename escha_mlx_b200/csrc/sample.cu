@@ -46,6 +46,7 @@ constexpr int kNear = 5;                    // bins around where a top-p cut is 
 constexpr int kSparse = 2048;               // listed tokens of a slice (16-bit places over the counts)
 constexpr float kCut = -30.0f;
 constexpr int kFraction = 44;
+constexpr double k512 = 738.65986093514925;  // 512 log2(e)
 static_assert(kThreads == 512 && kBins == 2 * kThreads,
               "one thread per entry of the table of powers, and per two bins");
 constexpr float kBinsPerNat = (kBins - 1) / 30.25f;
@@ -86,7 +87,7 @@ struct Shared {
     uint32_t cut_key;                       // (leader) the cut, for all CTAs
     uint32_t cut_ties;
     u64 bin_above;
-    u64 near[kNear + 2];                    // weights of the bins around a cut, before and behind
+    u64 near[kNear + 2];                    // weights of the bins around a cut, before them, of all
     u64 near_all[kNear + 2];                // the same of the row
     uint32_t warp_ties[kWarps];
     __align__(16) uint32_t hist[kBins];     // counts of this CTA
@@ -98,14 +99,12 @@ struct Shared {
 // Weight of a token in units of 2^-44.  2^(y / 512) = 2^(n / 512) * exp(r): a table for the
 // 512ths, a Taylor series of degree 3 for |r| <= ln 2 / 1024 (remainder below 9e-15).
 struct Weights {
-    double top, inv, inv512;                // 1 / T, and that times 512 log2(e)
-    float topf;
+    double top, inv512;                     // 512 log2(e) / T
     const double* pow2;
     __device__ __forceinline__ u64 operator()(float x) const {
         // no branches: the chains of several tokens overlap
-        const double d = static_cast<double>(x) - top;
-        const bool counts = d * inv >= static_cast<double>(kCut);
-        const double y = d * inv512;
+        const double y = (static_cast<double>(x) - top) * inv512;
+        const bool counts = y >= static_cast<double>(kCut) * k512;
         const double magic = 6755399441055744.0;                     // 1.5 * 2^52: rounds to integer
         const double shifted = y + magic;
         const int n = static_cast<int>(__double_as_longlong(shifted));
@@ -118,7 +117,7 @@ struct Weights {
         const double t = __longlong_as_double(__double_as_longlong(pow2[n & 511]) + scale);
         // t * e <= 2^44: adding 2^52 leaves the nearest integer in the low mantissa bits
         const u64 w = static_cast<u64>(__double_as_longlong(fma(t, e, 4503599627370496.0))) & 0xfffffffffffffull;
-        return x == topf ? 1ull << kFraction : counts ? w : 0ull;
+        return counts ? w : 0ull;
     }
 };
 
@@ -462,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 #pragma unroll
         for (int r = 0; r < kMaxCtas; ++r) best = o[r] > best ? o[r] : best;
     }
-    const float top = value_of(static_cast<uint32_t>(best >> 32));
+    float top = value_of(static_cast<uint32_t>(best >> 32));
     const int top_index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
     const bool empty = top == __int_as_float(0xff800000);
     if (empty || !(temperature > 0.0f)) {
@@ -475,17 +474,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const bool p_on = share0 < 1.0f, m_on = least > 0.0f;
     const u64 least_w = m_on ? static_cast<u64>(ceil(static_cast<double>(least) * (1ull << kFraction))) : 0;
 
+    auto value = [&](int i) { return to_float(xs[i]); };
+    if (top == __int_as_float(0x7f800000)) {
+        // infinite logits take everything: 0 where x is infinite, -inf elsewhere
+        __syncthreads();
+        for (int i = tid; i < p.slice; i += kThreads) xs[i] = value(i) == top ? T(0.0f) : lowest<T>();
+        if (most == top) most = 0.0f;
+        else most = __int_as_float(0xff800000);
+        top = 0.0f;
+        __syncthreads();
+    }
     Weights weight;
     weight.top = top;
-    weight.topf = top;
-    weight.inv = 1.0 / static_cast<double>(temperature);
-    weight.inv512 = weight.inv * 738.65986093514925;      // 512 log2(e)
+    weight.inv512 = k512 / static_cast<double>(temperature);
     weight.pow2 = s.pow2;
-    const float invf = 1.0f / temperature;
-    auto value = [&](int i) { return to_float(xs[i]); };
+    // bins of (top - x) / T; finite, so that the top itself has bin 0 at any temperature
+    const float bins = fminf(kBinsPerNat / temperature, 3e38f);
+    auto place_of = [&](float x) { return (top - x) * bins; };
     auto bin_of = [&](float x) {
-        if (x == top) return 0;
-        const float z = (top - x) * invf * kBinsPerNat;
+        const float z = place_of(x);
         return z < static_cast<float>(kBins - 1) ? static_cast<int>(z) : kBins - 1;
     };
     // token to take from a total, as a cumulative weight that has to be exceeded
@@ -513,6 +520,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         // tokens of bins [from, to] to the leader's list (as far as it has room)
         auto gather = [&](int from, int to) {
             if (__ballot_sync(0xffffffffu, my_bin <= to) == 0) return;
+            const float lowest_z = from, highest_z = min(to + 1, kBins - 1);
             // 64 tokens per thread and round: their hits as a mask, one reservation per warp
             constexpr int kRound = 64 / kVec;
             for (int v0 = 0; v0 < vecs; v0 += kRound * kThreads) {
@@ -527,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                         unsigned some = 0;
 #pragma unroll
                         for (int k = 0; k < kVec; ++k) {
-                            const int b = bin_of(to_float(e[k]));
-                            if (b >= from && b <= to && b < kBins - 1) some |= 1u << k;
+                            const float z = place_of(to_float(e[k]));
+                            if (z >= lowest_z && z < highest_z) some |= 1u << k;
                         }
                         hits |= static_cast<u64>(some) << (j * kVec);
                     }
@@ -620,8 +628,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
             for (int k = 0; k < kVec; ++k) {
-                const int b = bin_of(to_float(e[k]));
-                if (b < last) atomicAdd(&s.hist[b], 1u);
+                const float z = place_of(to_float(e[k]));
+                if (z < static_cast<float>(last)) atomicAdd(&s.hist[static_cast<int>(z)], 1u);
             }
         }
         cluster.sync();
@@ -767,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                         const uint32_t key = static_cast<uint32_t>(~x[e] >> 32);
                         const float v = value_of(key);
                         w[e] = i >= size ? 0 : by_count ? 1 : key >= cut_key ? weight(v) : 0;
-                        const float z = v == top ? 0.0f : (top - v) * invf * kBinsPerNat - static_cast<float>(bin);
+                        const float z = place_of(v) - static_cast<float>(bin);
                         sub[e] = min(max(static_cast<int>(z * kBins), 0), kBins - 1);
                     }
                     const u64 last_kept = locate(s, sub, x, w, goal - 1);
@@ -828,26 +836,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
             uint32_t* lo = s.work;
             if (tid < 2 * kNear) lo[tid] = 0;
             __syncthreads();
-            u64 ahead = 0, behind = 0;
+            u64 ahead = 0, whole = 0;
+            const float from = static_cast<float>(near_lo), upto = static_cast<float>(near_hi + 1);
             for (int v = first_vec + lane; v < last_vec; v += 32) {
                 const uint4 q = xv[v];
                 const T* e = reinterpret_cast<const T*>(&q);
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) {
-                    const float x = to_float(e[k]);
-                    const int b = bin_of(x);
+                    const float x = to_float(e[k]), z = place_of(x);
                     const u64 w = weight(x);
-                    ahead += b < near_lo ? w : 0;
-                    kept_ahead += b < near_lo && w >= least_w ? w : 0;
-                    behind += b > near_hi ? w : 0;
-                    if (b >= near_lo && b <= near_hi) Buckets{lo, lo + kNear}.add(b - near_lo, w);
+                    whole += w;
+                    if (z < from) ahead += w;
+                    if (m_on) kept_ahead += z < from && w >= least_w ? w : 0;
+                    if (z >= from && z < upto) Buckets{lo, lo + kNear}.add(static_cast<int>(z) - near_lo, w);
                 }
             }
+            if (!m_on) kept_ahead = ahead;
             ahead = warp_sum(ahead);
-            behind = warp_sum(behind);
+            whole = warp_sum(whole);
             if (lane == 0) {
                 s.warp_sum[warp] = ahead;
-                s.scan[warp] = behind;
+                s.scan[warp] = whole;
             }
             __syncthreads();
             if (tid < kNear) s.near[tid] = (static_cast<u64>(lo[kNear + tid]) << 32) + lo[tid];
@@ -866,8 +875,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
                 sums[tid] = t;
             }
             __syncthreads();
-            u64 before = sums[kNear], total = before + sums[kNear + 1];
-            for (int b = 0; b < kNear; ++b) total += sums[b];
+            u64 before = sums[kNear];
+            const u64 total = sums[kNear + 1];
             const double want_d = ceil(static_cast<double>(share) * static_cast<double>(total));
             u64 want = want_d > 1.0 ? static_cast<u64>(want_d) : 1ull;
             if (want > total) want = total;
@@ -976,8 +985,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 #pragma unroll
             for (int k = 0; k < kVec; ++k) {
                 const float x = to_float(e[k]);
-                const int b = bin_of(x);
-                if (b >= near_lo && b <= near_hi) sum += kept(x, weight(x), ties);
+                const float z = place_of(x);
+                if (z >= static_cast<float>(near_lo) && z < static_cast<float>(near_hi + 1))
+                    sum += kept(x, weight(x), ties);
             }
         }
     }
