@@ -927,13 +927,7 @@ int log_page_of(int page_size) {
     return -1;
 }
 
-int device_sms() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
-    return sms;
-}
+int device_sms() { return escha::sm_count(); }
 
 int check_cache(const char* fn, int H, int D, int page_size, int n_pages) {
     if (D != 64 && D != 128 && D != 256)
@@ -1053,7 +1047,8 @@ int escha_paged_attend(const void* q, long q_row, long q_head, int q_type, const
     REQUIRE_PTR(out);
     OPTIONAL_PTR(workspace);
     const int each = B < escha::kAttendMaxBatch ? B : escha::kAttendMaxBatch;
-    const escha::AttendShape s = escha::attend_shape(each, H, group, D, W, lp, device_sms());
+    const int sms = device_sms();
+    const escha::AttendShape s = escha::attend_shape(each, H, group, D, W, lp, sms);
     REQUIRE(((static_cast<long long>(W) << lp) / escha::kAttendBlock + 1) * each * H * s.chunks <
                 0x7fffffffll,
             "%s: %d requests of up to %lld tokens and %d heads are more than one launch numbers",
@@ -1074,15 +1069,16 @@ int escha_paged_attend(const void* q, long q_row, long q_head, int q_type, const
     p.H = H; p.group = group; p.chunks = s.chunks; p.heads = s.heads; p.D = D; p.W = W;
     p.log_page = lp; p.n_pages = n_pages;
     // larger batches take one launch after the other (each waits for the one before, so they
-    // share the workspace)
+    // share the workspace; a smaller last one needs no more of it)
     for (int b = 0; b < B; b += each) {
         p.B = B - b < each ? B - b : each;
-        p.ctas = escha::attend_shape(p.B, H, group, D, W, lp, device_sms()).ctas;
+        const escha::AttendShape now = escha::attend_shape(p.B, H, group, D, W, lp, sms);
+        p.ctas = now.ctas;
         p.q = static_cast<const char*>(q) + 2ll * b * q_row;
         p.out = static_cast<char*>(out) + 2ll * b * H * group * D;
         p.table = table + static_cast<long long>(b) * W;
         p.lengths = lengths + b;
-        const cudaError_t e = escha::launch_attend(p, q_type, cache_type, s.split, as_stream(stream));
+        const cudaError_t e = escha::launch_attend(p, q_type, cache_type, now.form, as_stream(stream));
         if (e != cudaSuccess) return cuda_result(e, "escha_paged_attend");
     }
     return ESCHA_OK;

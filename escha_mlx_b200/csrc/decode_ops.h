@@ -10,6 +10,9 @@ namespace escha {
 // Element types of the boundary (escha_b200.h: ESCHA_F16 ...).
 constexpr int kF16 = 0, kBF16 = 1, kF32 = 2, kI8 = 3;
 
+// Multiprocessors of the current device.
+int sm_count();
+
 constexpr int kPlanMaxBatch = 4096;
 
 struct PlanParams {
@@ -63,15 +66,18 @@ struct AttendParams {
     float scale_log2;        // score scale times log2(e)
     int B, H, group, chunks, heads, D, W, log_page, n_pages, ctas;
 };
+// How rows (a request's query heads of one key/value head) are shared out: a cluster each,
+// equal shares that cut rows (and a join), or equal shares that cannot.
+enum AttendForm { kAttendCluster, kAttendSplit, kAttendWhole };
 struct AttendShape {
+    AttendForm form;
     int heads;    // query heads of one work item: 8 or 16 at most
     int chunks;   // work items per key/value head
-    int ctas;     // CTAs of the launch
-    bool split;   // whether a row may be cut between CTAs at all
+    int ctas;     // CTAs per row (cluster), or of the launch
     size_t meta_bytes, ml_bytes, part_bytes;
 };
 AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, int sms);
-cudaError_t launch_attend(const AttendParams& p, int q_type, int cache_type, bool split,
+cudaError_t launch_attend(const AttendParams& p, int q_type, int cache_type, AttendForm form,
                           cudaStream_t st);
 
 struct SampleParams {

@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdlib>
 #include <cstring>
 #include <utility>
@@ -250,15 +251,19 @@ paged_append_kernel(const AppendParams p, int log_d8) {
     }
 }
 
+}  // namespace
+
 int sm_count() {
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int sms = known[dev].load(std::memory_order_relaxed);
+    if (sms == 0) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+        known[dev].store(sms, std::memory_order_relaxed);
+    }
     return sms;
 }
-
-}  // namespace
 
 cudaError_t launch_page_plan(const PlanParams& p, cudaStream_t st) {
     const int most = (p.rows + kPlanThreads - 1) / kPlanThreads;

@@ -29,9 +29,12 @@
 // Split.  The work is a line of blocks of 64 tokens, over all requests and key/value heads;
 // each CTA takes an equal share of it, whatever the lengths are, and cuts rows where its share
 // ends.  A CTA leaves at most two unfinished rows (its first and its last); a second, chained
-// kernel joins the pieces of each row in order.  No counters, nothing to clear.
+// kernel joins the pieces of each row in order.  No counters, nothing to clear.  Where all rows
+// fit the GPU at once and none can be long, a row is cut between the CTAs of a cluster instead,
+// which join through distributed shared memory: one launch and no scratch.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -46,9 +49,12 @@
 namespace escha {
 namespace attend {
 
+namespace cg = cooperative_groups;
+
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;
+constexpr int kMaxCluster = 8;
 static_assert(kTile * kWarps == kAttendBlock, "a block is one tile per warp");
 
 // A lane's copy of N bytes, completed by cp.async.wait_group; bytes past `have` are zeros.
@@ -181,7 +187,8 @@ __device__ __forceinline__ void block_counts(const AttendParams& p, int* s_prefi
     __syncthreads();
 }
 
-template <bool QBF, bool I8, int D, int NT>
+// CL: a row per cluster of p.ctas CTAs; otherwise equal shares of all blocks, p.ctas of them.
+template <bool QBF, bool I8, int D, int NT, bool CL>
 __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p) {
     using S = Shape<QBF, I8, D, NT>;
     constexpr bool BF = S::kBF;
@@ -195,31 +202,34 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
     float* s_l = s_m + kWarps * S::kHeads;
     float* s_qscale = s_l + kWarps * S::kHeads;
     int* s_sums = reinterpret_cast<int*>(s_qscale + S::kHeads);
+    float* s_part = reinterpret_cast<float*>(s_prefix);   // CL: maximum and sum by head
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     grid_launch_dependents();
     grid_dependency_wait();
-    block_counts(p, s_prefix, s_sums);
+    if constexpr (!CL) block_counts(p, s_prefix, s_sums);
 
     const int per_request = p.H * p.chunks;               // rows of a request
-    const long long total = static_cast<long long>(s_prefix[p.B]) * per_request;
     const int c = blockIdx.x;
-    // as many CTAs as there are blocks at most, so that no share is empty
-    const long long shares = min(static_cast<long long>(p.ctas), total);
-    long long u = c < shares ? total * c / shares : 0;
-    const long long u_end = c < shares ? total * (c + 1) / shares : 0;
     using QT = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
     const QT* q = static_cast<const QT*>(p.q);
     QT* out = static_cast<QT*>(p.out);
     const int heads_total = p.H * p.group;
-
-    // requests without a token: zeros
-    for (int b = c; b < p.B; b += p.ctas)
-        if (s_prefix[b + 1] == s_prefix[b])
-            for (int i = tid; i < heads_total * D / 8; i += kThreads)
-                reinterpret_cast<uint4*>(out + static_cast<size_t>(b) * heads_total * D)[i] =
-                    make_uint4(0, 0, 0, 0);
+    long long total = 0, shares = 0, u = 0, u_end = 1;
+    if constexpr (!CL) {
+        total = static_cast<long long>(s_prefix[p.B]) * per_request;
+        // as many CTAs as there are blocks at most, so that no share is empty
+        shares = min(static_cast<long long>(p.ctas), total);
+        u = c < shares ? total * c / shares : 0;
+        u_end = c < shares ? total * (c + 1) / shares : 0;
+        // requests without a token: zeros
+        for (int b = c; b < p.B; b += p.ctas)
+            if (s_prefix[b + 1] == s_prefix[b])
+                for (int i = tid; i < heads_total * D / 8; i += kThreads)
+                    reinterpret_cast<uint4*>(out + static_cast<size_t>(b) * heads_total * D)[i] =
+                        make_uint4(0, 0, 0, 0);
+    }
     int unfinished_row = -1, unfinished_last = -1;
 
     const uint32_t ring = smem_u32(s_body) + warp * (S::kStages * S::kRingStage);
@@ -228,22 +238,33 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
     const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
 
     while (u < u_end) {
-        // the row that holds block u
-        int lo = 0, hi = p.B;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (static_cast<long long>(s_prefix[mid]) * per_request <= u) lo = mid; else hi = mid;
+        int b, rr, k0, k1, blocks, len;                   // rr: head and chunk
+        if constexpr (CL) {
+            const int row = c / p.ctas, part = c - row * p.ctas;
+            b = row / per_request;
+            rr = row - b * per_request;
+            len = min(max(p.lengths[b], 0), p.W << p.log_page);
+            blocks = (len + kAttendBlock - 1) / kAttendBlock;
+            k0 = blocks * part / p.ctas;
+            k1 = blocks * (part + 1) / p.ctas;
+        } else {
+            // the row that holds block u
+            int hi = p.B;
+            b = 0;
+            while (hi - b > 1) {
+                const int mid = (b + hi) >> 1;
+                if (static_cast<long long>(s_prefix[mid]) * per_request <= u) b = mid; else hi = mid;
+            }
+            blocks = s_prefix[b + 1] - s_prefix[b];
+            const int in_request = static_cast<int>(u - static_cast<long long>(s_prefix[b]) * per_request);
+            rr = in_request / blocks;
+            k0 = in_request - rr * blocks;
+            k1 = static_cast<int>(min(static_cast<long long>(blocks), k0 + (u_end - u)));
+            len = min(max(p.lengths[b], 0), p.W << p.log_page);
         }
-        const int b = lo;
-        const int blocks = s_prefix[b + 1] - s_prefix[b];
-        const int in_request = static_cast<int>(u - static_cast<long long>(s_prefix[b]) * per_request);
-        const int rr = in_request / blocks;               // head and chunk
-        const int k0 = in_request - rr * blocks;
-        const int k1 = static_cast<int>(min(static_cast<long long>(blocks), k0 + (u_end - u)));
         const int h = rr / p.chunks, chunk = rr - h * p.chunks;
         const int head0 = h * p.group + chunk * S::kHeads;
         const int nheads = min(S::kHeads, p.group - chunk * S::kHeads);
-        const int len = min(max(p.lengths[b], 0), p.W << p.log_page);
         const int t0 = k0 * kAttendBlock, t1 = min(len, k1 * kAttendBlock);
         const bool starts = k0 == 0, ends = k1 == blocks;
         const int32_t* pages = p.table + static_cast<size_t>(b) * p.W;
@@ -580,7 +601,14 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
                 o.z += a * x.z;
                 o.w += a * x.w;
             }
-            if (starts && ends) {
+            if (CL && p.ctas > 1) {
+                // the CTA's sums in place of the first warp's
+                *reinterpret_cast<float4*>(s_acc + head * (D + 4) + d) = o;
+                if (d == 0) {
+                    s_part[2 * head] = top;
+                    s_part[2 * head + 1] = sum;
+                }
+            } else if (CL || (starts && ends)) {
                 // nothing to attend to (no usable page): zeros
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 QT* dst = out + (static_cast<size_t>(b) * heads_total + head0 + head) * D + d;
@@ -591,6 +619,47 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
                 *reinterpret_cast<float4*>(p.part + at * D + d) = o;
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(top, sum);
             }
+        }
+        if constexpr (CL) {
+            if (p.ctas > 1) {
+                cg::cluster_group cluster = cg::this_cluster();
+                cluster.sync();
+                const int items = nheads * (D / 4);
+                for (int i = cluster.block_rank() * kThreads + tid; i < items; i += p.ctas * kThreads) {
+                    const int head = i / (D / 4), d = (i % (D / 4)) * 4;
+                    float2 ml[kMaxCluster];
+                    float4 x[kMaxCluster];
+#pragma unroll
+                    for (int r = 0; r < kMaxCluster; ++r)
+                        if (r < p.ctas) {
+                            ml[r] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(s_part, r) + 2 * head);
+                            x[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_acc, r) + head * (D + 4) + d);
+                        }
+                    float top = ml[0].x;
+#pragma unroll
+                    for (int r = 1; r < kMaxCluster; ++r)
+                        if (r < p.ctas) top = fmaxf(top, ml[r].x);
+                    const float ref = top == __int_as_float(0xff800000) ? 0.0f : top;
+                    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < kMaxCluster; ++r)
+                        if (r < p.ctas) {
+                            const float a = exp2_approx(ml[r].x - ref);
+                            sum += a * ml[r].y;
+                            o.x += a * x[r].x;
+                            o.y += a * x[r].y;
+                            o.z += a * x[r].z;
+                            o.w += a * x[r].w;
+                        }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    QT* dst = out + (static_cast<size_t>(b) * heads_total + head0 + head) * D + d;
+                    *reinterpret_cast<uint2*>(dst) =
+                        make_uint2(pack2<QBF>(o.x * inv, o.y * inv), pack2<QBF>(o.z * inv, o.w * inv));
+                }
+                cluster.sync();                           // no CTA leaves while its sums are read
+            }
+            return;
         }
         if (starts && !ends) {
             unfinished_row = b * per_request + rr;
@@ -689,28 +758,48 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendP
 }
 
 template <bool QBF, bool I8, int D, int NT>
-cudaError_t launch(const AttendParams& p, bool split, cudaStream_t st) {
+cudaError_t launch(const AttendParams& p, AttendForm form, cudaStream_t st) {
     using S = Shape<QBF, I8, D, NT>;
+    if (form == kAttendCluster) {
+        static SmemLimit limit;
+        cudaError_t e = limit.ensure(attend_kernel<QBF, I8, D, NT, true>, S::kShared);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(p.B * p.H * p.chunks * p.ctas);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = S::kShared;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.ctas;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_allowed() ? 2 : 1;
+        return cudaLaunchKernelEx(&cfg, attend_kernel<QBF, I8, D, NT, true>, p);
+    }
     static SmemLimit limit;
-    cudaError_t e = limit.ensure(attend_kernel<QBF, I8, D, NT>, S::kShared);
+    cudaError_t e = limit.ensure(attend_kernel<QBF, I8, D, NT, false>, S::kShared);
     if (e != cudaSuccess) return e;
-    e = launch_chained(attend_kernel<QBF, I8, D, NT>, dim3(p.ctas), dim3(kThreads), S::kShared, st, p);
-    if (e != cudaSuccess || !split) return e;
+    e = launch_chained(attend_kernel<QBF, I8, D, NT, false>, dim3(p.ctas), dim3(kThreads), S::kShared, st, p);
+    if (e != cudaSuccess || form == kAttendWhole) return e;
     const size_t smem = (((p.ctas + 3) & ~3) + kJoinThreads / (D / 4) * D) * sizeof(float);
     return launch_chained(attend_join_kernel<QBF, D>, dim3(p.ctas, p.heads), dim3(kJoinThreads), smem,
                           st, p);
 }
 
 template <bool QBF, bool I8>
-cudaError_t launch_any(const AttendParams& p, bool split, cudaStream_t st) {
+cudaError_t launch_any(const AttendParams& p, AttendForm form, cudaStream_t st) {
     if (p.heads == 8) {
-        if (p.D == 64) return launch<QBF, I8, 64, 1>(p, split, st);
-        if (p.D == 128) return launch<QBF, I8, 128, 1>(p, split, st);
-        return launch<QBF, I8, 256, 1>(p, split, st);
+        if (p.D == 64) return launch<QBF, I8, 64, 1>(p, form, st);
+        if (p.D == 128) return launch<QBF, I8, 128, 1>(p, form, st);
+        return launch<QBF, I8, 256, 1>(p, form, st);
     }
-    if (p.D == 64) return launch<QBF, I8, 64, 2>(p, split, st);
-    if (p.D == 128) return launch<QBF, I8, 128, 2>(p, split, st);
-    return launch<QBF, I8, 256, 2>(p, split, st);
+    if (p.D == 64) return launch<QBF, I8, 64, 2>(p, form, st);
+    if (p.D == 128) return launch<QBF, I8, 128, 2>(p, form, st);
+    return launch<QBF, I8, 256, 2>(p, form, st);
 }
 
 }  // namespace attend

@@ -3,6 +3,6 @@
 
 namespace escha {
 namespace attend {
-template cudaError_t launch_any<false, false>(const AttendParams&, bool, cudaStream_t);
+template cudaError_t launch_any<false, false>(const AttendParams&, AttendForm, cudaStream_t);
 }  // namespace attend
 }  // namespace escha
