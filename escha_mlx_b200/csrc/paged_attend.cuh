@@ -12,8 +12,8 @@
 // the 8 columns.  The order of the summed index is free, so lane (g, t) = (lane / 4, lane % 4)
 // takes 16 contiguous bytes of token rows g and g + 8 for the first product, and contiguous
 // bytes of token rows 2t, 2t + 1, 2t + 8, 2t + 9 for the second, whose pairs along the tokens
-// are put together by byte permutes.  Each warp has a ring of its own (key tile, value tile,
-// key tile, ... of 16 tokens) that it fills with cp.async, 512 contiguous bytes of the cache
+// are put together by byte permutes.  Each warp has a ring of its own (keys, values,
+// keys, ... of 16 to 64 tokens) that it fills with cp.async, 512 contiguous bytes of the cache
 // per instruction: fetching each lane's own operand bytes instead (64-byte runs) needed no
 // exchange between lanes but ran at 4.9 TB/s against 6.8.  The 16-byte pieces of a tile are
 // stored with an exclusive-or swizzle under which the fill and both operand reads are free of
@@ -53,9 +53,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = 16;
 constexpr int kMaxCluster = 8;
-static_assert(kTile * kWarps == kAttendBlock, "a block is one tile per warp");
 
 // A lane's copy of N bytes, completed by cp.async.wait_group; bytes past `have` are zeros.
 template <int N>
@@ -132,25 +130,32 @@ template <> struct Words<4> { uint32_t v; __device__ uint32_t operator[](int) co
 template <bool QBF, bool I8, int D, int NT>
 struct Shape {
     static constexpr bool kBF = QBF && !I8;               // type of the products
+    static constexpr int kResident = 2;                   // CTAs that share an SM
     static constexpr int kElem = I8 ? 1 : 2;
     static constexpr int kRow = D * kElem;                // bytes of a token's row
     static constexpr int kChunks = kRow / 64;             // 64-byte pieces of a row
-    static constexpr int kHalf = kTile * kRow;            // bytes of a key or value tile
-    // depth of a warp's ring: two or three tiles ahead, whatever their size
-    static constexpr int kStages = kHalf >= 8192 ? 3 : kHalf >= 4096 ? (I8 ? 5 : 6) : 8;
+    // A warp's step takes kSubs tiles of 16 tokens: with short rows the softmax around a single
+    // one (exchanges, votes) would take longer than its bytes.
+    static constexpr int kSubs = NT == 2 ? (kRow <= 128 ? 2 : 1) : kRow >= 512 ? 1 : kRow == 256 ? 2 : 4;
+    static constexpr int kTile = 16 * kSubs;
+    static constexpr int kHalf = kTile * kRow;            // bytes of a step's keys or values
     static constexpr int kSets = kRow == 512 ? 2 : 1;     // value rows as 16 pieces per set
     static constexpr int kPiece = kRow / kSets / 16;      // bytes of a piece: 16, 8 or 4
     static constexpr int kPerPiece = kPiece / kElem;      // channels of a piece
     static constexpr int kMma = kSets * kPerPiece;        // O^T tiles of 16 channels
-    static constexpr int kScales = I8 ? 2 * kTile * 4 : 0;   // bytes of a tile's scales in the ring
+    static constexpr int kScales = I8 ? 2 * kTile * 4 : 0;   // bytes of a step's scales in the ring
     static constexpr int kQWords = I8 ? 8 : 4;            // query words per lane and chunk
     static constexpr int kQBytes = NT * kChunks * kQWords * 4 * 32;
     static constexpr int kRingStage = kHalf + kScales;
-    static constexpr int kRing = kWarps * kStages * kRingStage;
     static constexpr int kHeads = 8 * NT;
+    static constexpr int kFixed = (kAttendMaxBatch + 4) * 4 + 2 * kWarps * kHeads * 4 + kHeads * 4 + 64;
+    // depth of a warp's ring: what the CTAs that share an SM leave
+    static constexpr int kMost = (226 * 1024 / kResident - 1024 - kFixed - kQBytes) / (kWarps * kRingStage);
+    static constexpr int kStages = kMost > 8 ? 8 : kMost;
+    static_assert(kStages >= 3, "a step's keys and values in flight beside what is in use");
+    static constexpr int kRing = kWarps * kStages * kRingStage;
     static constexpr int kJoin = kWarps * kHeads * (D + 4) * 4;   // the warps' sums, over the ring
     static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
-    static constexpr int kFixed = (kAttendMaxBatch + 4) * 4 + 2 * kWarps * kHeads * 4 + kHeads * 4 + 64;
     static constexpr int kShared = kBody + kQBytes + kFixed;
 };
 
@@ -189,7 +194,7 @@ __device__ __forceinline__ void block_counts(const AttendParams& p, int* s_prefi
 
 // CL: a row per cluster of p.ctas CTAs; otherwise equal shares of all blocks, p.ctas of them.
 template <bool QBF, bool I8, int D, int NT, bool CL>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) attend_kernel(const AttendParams p) {
     using S = Shape<QBF, I8, D, NT>;
     constexpr bool BF = S::kBF;
     // power of two on the weights (binary16 products only)
@@ -270,21 +275,24 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
         const int32_t* pages = p.table + static_cast<size_t>(b) * p.W;
 
         // tiles of this warp: warp, warp + kWarps, ... of the segment
+        constexpr int kSubs = S::kSubs, kTile = S::kTile;
         const int tiles = (t1 - t0 + kTile - 1) / kTile;
         const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
         const int halves = 2 * mine;                      // K0, V0, K1, V1, ...
-        int ids = -1;                                     // lane j: page of tile j (mod 32)
-        uint32_t bad = 0;                                 // tiles (mod 32) without a usable page
-        const uint8_t *k_src = kc, *v_src = vc;           // first token of the tile being fetched
-        const float *ks_src = p.k_scale, *vs_src = p.v_scale;
-        int k_have = 0;                                   // its tokens
-        auto fetch_rows = [&](uint32_t dst, const uint8_t* src) {
+        int ids = -1;                                     // lane j: page of the 16 tokens j (mod 32)
+        uint32_t bad = 0;                                 // those (mod 32) without a usable page
+        size_t rows[kSubs];                               // cache rows of the step being fetched
+        int have[kSubs];                                  // and its tokens, by 16
+        auto fetch_rows = [&](uint32_t dst, const uint8_t* cache) {
 #pragma unroll
             for (int x = 0; x < S::kHalf / 512; ++x) {
-                const int r = x * (512 / S::kRow) + lane / (S::kRow / 16);
+                constexpr int kRows = 512 / S::kRow;      // rows per instruction, of one 16
+                const int m = x * kRows / 16;
+                const int r = x * kRows % 16 + lane / (S::kRow / 16);
                 const int byte = lane % (S::kRow / 16) * 16;
-                const bool in = r < k_have;
-                copy_async<16>(dst + place<S::kRow>(r, byte), src + (in ? r * S::kRow + byte : 0), in ? 16 : 0);
+                const bool in = r < have[m];
+                copy_async<16>(dst + place<S::kRow>(m * 16 + r, byte),
+                               cache + rows[m] * S::kRow + (in ? r * S::kRow + byte : 0), in ? 16 : 0);
             }
         };
         auto fetch = [&](int i, int stage) {
@@ -292,32 +300,31 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
                 const int j = i >> 1;
                 const uint32_t dst = ring + stage * S::kRingStage;
                 if ((i & 1) == 0) {
-                    if ((j & 31) == 0) {
-                        const int tok = t0 + kTile * (warp + kWarps * (j + lane));
+                    if ((j * kSubs & 31) == 0) {
+                        const int tok = t0 + kTile * (warp + kWarps * (j + lane / kSubs)) + lane % kSubs * 16;
                         ids = tok < t1 ? pages[tok >> p.log_page] : -1;
                     }
-                    const int page = __shfl_sync(0xffffffffu, ids, j & 31);
-                    const int tok = t0 + kTile * (warp + kWarps * j);
-                    const bool ok = page >= 0 && page < p.n_pages;
-                    bad = (bad & ~(1u << (j & 31))) | (ok ? 0u : 1u << (j & 31));
-                    k_have = ok ? min(kTile, t1 - tok) : 0;
-                    const size_t row = (((ok ? static_cast<size_t>(page) : 0) * p.H + h) << p.log_page) +
-                                       (tok & ((1 << p.log_page) - 1));
-                    k_src = kc + row * S::kRow;
-                    v_src = vc + row * S::kRow;
-                    if constexpr (I8) {
-                        ks_src = p.k_scale + row;
-                        vs_src = p.v_scale + row;
+#pragma unroll
+                    for (int m = 0; m < kSubs; ++m) {
+                        const int at = (j * kSubs + m) & 31;
+                        const int page = __shfl_sync(0xffffffffu, ids, at);
+                        const int tok = t0 + kTile * (warp + kWarps * j) + 16 * m;
+                        const bool ok = page >= 0 && page < p.n_pages;
+                        bad = (bad & ~(1u << at)) | (ok ? 0u : 1u << at);
+                        have[m] = ok ? min(16, t1 - tok) : 0;
+                        rows[m] = (((ok ? static_cast<size_t>(page) : 0) * p.H + h) << p.log_page) +
+                                  (tok & ((1 << p.log_page) - 1));
+                        if constexpr (I8) {
+                            // scales: lanes 0..15 K's, the others V's
+                            const float* src = (lane < 16 ? p.k_scale : p.v_scale) + rows[m];
+                            const bool in = (lane & 15) < have[m];
+                            copy_async<4>(dst + S::kHalf + (m * 32 + lane) * 4, src + (in ? lane & 15 : 0),
+                                          in ? 4 : 0);
+                        }
                     }
-                    fetch_rows(dst, k_src);
-                    if constexpr (I8) {
-                        // scales: lanes 0..15 K's, the others V's
-                        const float* src = lane < kTile ? ks_src : vs_src;
-                        const bool in = (lane & 15) < k_have;
-                        copy_async<4>(dst + S::kHalf + lane * 4, src + (in ? lane & 15 : 0), in ? 4 : 0);
-                    }
+                    fetch_rows(dst, kc);
                 } else {
-                    fetch_rows(dst, v_src);
+                    fetch_rows(dst, vc);
                 }
             }
             cp_async_commit();
@@ -381,99 +388,119 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
         }
 
         float acc[NT][S::kMma][4];
-        float m[NT][2], l[NT][2];
+        float m_run[NT][2], l[NT][2];                     // running maxima; sums by lane
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int k = 0; k < S::kMma; ++k)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[nt][k][e] = 0.0f;
-            m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
+            m_run[nt][0] = m_run[nt][1] = __int_as_float(0xff800000);
             l[nt][0] = l[nt][1] = 0.0f;
         }
 
         int rd = 0, wr = S::kStages - 1;                  // stages to read and to fill next
         for (int j = 0; j < mine; ++j) {
-            // ---- scores of 16 tokens
+            // ---- scores of the step's tokens
             cp_async_wait<S::kStages - 2>();
             __syncwarp();         // the other lanes' copies; their reads of the stage to fill next
             const uint8_t* tile = ring_ptr + rd * S::kRingStage;
-            float s[NT][4], s2[NT][4];
+            // two chains of products where the step has one tile only
+            constexpr int kChains = kSubs == 1 ? 2 : 1;
+            float s[NT][kSubs][kChains][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
+                for (int m = 0; m < kSubs; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4 * kChains; ++e) s[nt][m][e >> 2][e & 3] = 0.0f;
 #pragma unroll
             for (int x = 0; x < S::kChunks; ++x) {
-                Words<16> r0, r1;
-                r0.v = *reinterpret_cast<const uint4*>(tile + place<S::kRow>(g, x * 64 + t * 16));
-                r1.v = *reinterpret_cast<const uint4*>(tile + place<S::kRow>(g + 8, x * 64 + t * 16));
+                constexpr int kPer = S::kQWords / 4;
+                Words<16> qa[NT], qb[NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    Words<16> qa, qb;
-                    constexpr int kPer = S::kQWords / 4;
-                    qa.v = reinterpret_cast<const uint4*>(s_q)[((nt * S::kChunks + x) * kPer) * 32 + lane];
+                    qa[nt].v = reinterpret_cast<const uint4*>(s_q)[((nt * S::kChunks + x) * kPer) * 32 + lane];
+                    if constexpr (I8)
+                        qb[nt].v = reinterpret_cast<const uint4*>(s_q)[((nt * S::kChunks + x) * kPer + 1) * 32 + lane];
+                }
+#pragma unroll
+                for (int m = 0; m < kSubs; ++m) {
+                    Words<16> r0, r1;
+                    r0.v = *reinterpret_cast<const uint4*>(tile + place<S::kRow>(m * 16 + g, x * 64 + t * 16));
+                    r1.v = *reinterpret_cast<const uint4*>(tile + place<S::kRow>(m * 16 + g + 8, x * 64 + t * 16));
                     if constexpr (!I8) {
-                        mma<BF>(s[nt], r0[0], r1[0], r0[1], r1[1], qa[0], qa[1]);
-                        mma<BF>(s2[nt], r0[2], r1[2], r0[3], r1[3], qa[2], qa[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<BF>(s[nt][m][0], r0[0], r1[0], r0[1], r1[1], qa[nt][0], qa[nt][1]);
+                            mma<BF>(s[nt][m][kChains - 1], r0[2], r1[2], r0[3], r1[3], qa[nt][2], qa[nt][3]);
+                        }
                     } else {
-                        qb.v = reinterpret_cast<const uint4*>(s_q)[((nt * S::kChunks + x) * kPer + 1) * 32 + lane];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t a = r0[k] ^ 0x80808080u, e = r1[k] ^ 0x80808080u;
-                            mma<false>(k & 1 ? s2[nt] : s[nt], codes_f16<0x4140>(a), codes_f16<0x4140>(e),
-                                       codes_f16<0x4342>(a), codes_f16<0x4342>(e),
-                                       k < 2 ? qa[2 * k] : qb[2 * k - 4], k < 2 ? qa[2 * k + 1] : qb[2 * k - 3]);
+                            const uint32_t a0 = codes_f16<0x4140>(a), a1 = codes_f16<0x4140>(e);
+                            const uint32_t a2 = codes_f16<0x4342>(a), a3 = codes_f16<0x4342>(e);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                mma<false>(s[nt][m][k & (kChains - 1)], a0, a1, a2, a3,
+                                           k < 2 ? qa[nt][2 * k] : qb[nt][2 * k - 4],
+                                           k < 2 ? qa[nt][2 * k + 1] : qb[nt][2 * k - 3]);
                         }
                     }
                 }
             }
-            float4 sc = make_float4(1.0f, 1.0f, 1.0f, 1.0f);   // K's, then V's scales of tokens g, g + 8
+            // K's, then V's scales of tokens g, g + 8
+            float4 sc[I8 ? kSubs : 1];
             if constexpr (I8) {
                 const float* scales = reinterpret_cast<const float*>(tile + S::kHalf);
-                sc = make_float4(scales[g], scales[g + 8], scales[kTile + g], scales[kTile + g + 8]);
+#pragma unroll
+                for (int m = 0; m < kSubs; ++m)
+                    sc[m] = make_float4(scales[m * 32 + g], scales[m * 32 + g + 8], scales[m * 32 + 16 + g],
+                                        scales[m * 32 + 24 + g]);
             }
             fetch(2 * j + S::kStages - 1, wr);
             rd = rd + 1 == S::kStages ? 0 : rd + 1;
             wr = wr + 1 == S::kStages ? 0 : wr + 1;
 
             // ---- weights
-            const int tok = t0 + kTile * (warp + kWarps * j);
-            const int have = (bad >> (j & 31)) & 1 ? 0 : min(kTile, t1 - tok);
-            uint32_t hi0[NT], hi1[NT], lo0[NT], lo1[NT];
+            const int left = t1 - (t0 + kTile * (warp + kWarps * j));
+            uint32_t hi0[NT][kSubs], hi1[NT][kSubs], lo0[NT][kSubs], lo1[NT][kSubs];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float x[4];
+                float x[kSubs][4], up[2];
+                up[0] = up[1] = __int_as_float(0xff800000);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float y = s[nt][e] + s2[nt][e];
-                    if constexpr (I8) y *= e < 2 ? sc.x : sc.y;
-                    y *= qs[nt][e & 1];
-                    x[e] = g + (e < 2 ? 0 : 8) < have ? y : __int_as_float(0xff800000);
-                }
-                float up[2];
-                if constexpr (I8) {
-                    // exponents of V's scales, so that weight times scale stays at most 2
-                    const float e0 = static_cast<float>(max((__float_as_int(sc.z) >> 23) - 127, -90));
-                    const float e1 = static_cast<float>(max((__float_as_int(sc.w) >> 23) - 127, -90));
-                    up[0] = fmaxf(x[0] + e0, x[2] + e1);
-                    up[1] = fmaxf(x[1] + e0, x[3] + e1);
-                } else {
-                    up[0] = fmaxf(x[0], x[2]);
-                    up[1] = fmaxf(x[1], x[3]);
+                for (int m = 0; m < kSubs; ++m) {
+                    const int usable = (bad >> ((j * kSubs + m) & 31)) & 1 ? 0 : left - 16 * m;
+                    float above[2] = {0.0f, 0.0f};
+                    if constexpr (I8) {
+                        // exponents of V's scales, so that weight times scale stays at most 2
+                        above[0] = static_cast<float>(max((__float_as_int(sc[m].z) >> 23) - 127, -90));
+                        above[1] = static_cast<float>(max((__float_as_int(sc[m].w) >> 23) - 127, -90));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float y = s[nt][m][0][e];
+                        if constexpr (kChains == 2) y += s[nt][m][1][e];
+                        if constexpr (I8) y *= e < 2 ? sc[m].x : sc[m].y;
+                        y *= qs[nt][e & 1];
+                        x[m][e] = g + (e < 2 ? 0 : 8) < usable ? y : __int_as_float(0xff800000);
+                        up[e & 1] = fmaxf(up[e & 1], I8 ? x[m][e] + above[e >> 1] : x[m][e]);
+                    }
                 }
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
                     up[0] = fmaxf(up[0], __shfl_xor_sync(0xffffffffu, up[0], d));
                     up[1] = fmaxf(up[1], __shfl_xor_sync(0xffffffffu, up[1], d));
                 }
-                const bool raise = up[0] > m[nt][0] || up[1] > m[nt][1];
+                const bool raise = up[0] > m_run[nt][0] || up[1] > m_run[nt][1];
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float to = fmaxf(m[nt][e], up[e]);
-                        const float a = to == __int_as_float(0xff800000) ? 1.0f : exp2_approx(m[nt][e] - to);
-                        m[nt][e] = to;
+                        const float to = fmaxf(m_run[nt][e], up[e]);
+                        const float a = to == __int_as_float(0xff800000) ? 1.0f : exp2_approx(m_run[nt][e] - to);
+                        m_run[nt][e] = to;
                         l[nt][e] *= a;
 #pragma unroll
                         for (int k = 0; k < S::kMma; ++k) {
@@ -482,24 +509,28 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
                         }
                     }
                 }
-                float w[4];
+                // no finite score yet: every weight is zero
+                const float ref0 = m_run[nt][0] == __int_as_float(0xff800000) ? 0.0f : m_run[nt][0] - kLift;
+                const float ref1 = m_run[nt][1] == __int_as_float(0xff800000) ? 0.0f : m_run[nt][1] - kLift;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // no finite score yet: every weight of the tile is zero
-                    const float ref = m[nt][e & 1] == __int_as_float(0xff800000) ? 0.0f : m[nt][e & 1] - kLift;
-                    w[e] = exp2_approx(x[e] - ref);
-                    l[nt][e & 1] += w[e];
-                    if constexpr (I8) {
-                        // a masked token's scale is zero-filled: 0 * 0
-                        w[e] *= e < 2 ? sc.z : sc.w;
+                for (int m = 0; m < kSubs; ++m) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = exp2_approx(x[m][e] - (e & 1 ? ref1 : ref0));
+                        l[nt][e & 1] += w[e];
+                        if constexpr (I8) {
+                            // a masked token's scale is zero-filled: 0 * 0
+                            w[e] *= e < 2 ? sc[m].z : sc[m].w;
+                        }
                     }
+                    const uint32_t h0 = pack2<BF>(w[0], w[1]), h1 = pack2<BF>(w[2], w[3]);
+                    const float2 f0 = unpack2<BF>(h0), f1 = unpack2<BF>(h1);
+                    hi0[nt][m] = transpose8(h0);
+                    hi1[nt][m] = transpose8(h1);
+                    lo0[nt][m] = transpose8(pack2<BF>(w[0] - f0.x, w[1] - f0.y));
+                    lo1[nt][m] = transpose8(pack2<BF>(w[2] - f1.x, w[3] - f1.y));
                 }
-                const uint32_t h0 = pack2<BF>(w[0], w[1]), h1 = pack2<BF>(w[2], w[3]);
-                const float2 f0 = unpack2<BF>(h0), f1 = unpack2<BF>(h1);
-                hi0[nt] = transpose8(h0);
-                hi1[nt] = transpose8(h1);
-                lo0[nt] = transpose8(pack2<BF>(w[0] - f0.x, w[1] - f0.y));
-                lo1[nt] = transpose8(pack2<BF>(w[2] - f1.x, w[3] - f1.y));
             }
 
             // ---- weighted values
@@ -507,46 +538,45 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
             __syncwarp();
             tile = ring_ptr + rd * S::kRingStage;
 #pragma unroll
-            for (int z = 0; z < S::kSets; ++z) {
-                Words<S::kPiece> v[2][4];                 // piece g, g + 8; tokens 2t, 2t+1, 2t+8, 2t+9
+            for (int m = 0; m < kSubs; ++m)
 #pragma unroll
-                for (int y = 0; y < 8; ++y)
-                    v[y >> 2][y & 3].v = *reinterpret_cast<const decltype(v[0][0].v)*>(
-                        tile + place<S::kRow>(2 * t + (y & 1) + (y & 2) * 4,
-                                              (z * 16 + (y >> 2) * 8 + g) * S::kPiece));
+                for (int z = 0; z < S::kSets; ++z) {
+                    Words<S::kPiece> v[2][4];             // piece g, g + 8; tokens 2t, 2t+1, 2t+8, 2t+9
 #pragma unroll
-                for (int w = 0; w < S::kPiece / 4; ++w) {
-                    uint32_t a[4][I8 ? 4 : 2];            // operand registers of the word's channels
-                    if constexpr (!I8) {
+                    for (int y = 0; y < 8; ++y)
+                        v[y >> 2][y & 3].v = *reinterpret_cast<const decltype(v[0][0].v)*>(
+                            tile + place<S::kRow>(m * 16 + 2 * t + (y & 1) + (y & 2) * 4,
+                                                  (z * 16 + (y >> 2) * 8 + g) * S::kPiece));
+#pragma unroll
+                    for (int w = 0; w < S::kPiece / 4; ++w) {
+                        uint32_t a[4][I8 ? 4 : 2];        // operand registers of the word's channels
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {     // r: (piece, token pair) in A's order
-                            const uint32_t v0 = v[r & 1][(r >> 1) * 2][w], v1 = v[r & 1][(r >> 1) * 2 + 1][w];
-                            a[r][0] = __byte_perm(v0, v1, 0x5410);
-                            a[r][1] = __byte_perm(v0, v1, 0x7632);
+                            uint32_t v0 = v[r & 1][(r >> 1) * 2][w], v1 = v[r & 1][(r >> 1) * 2 + 1][w];
+                            if constexpr (!I8) {
+                                a[r][0] = __byte_perm(v0, v1, 0x5410);
+                                a[r][1] = __byte_perm(v0, v1, 0x7632);
+                            } else {
+                                v0 ^= 0x80808080u;
+                                v1 ^= 0x80808080u;
+                                const uint32_t p01 = __byte_perm(v0, v1, 0x5140), p23 = __byte_perm(v0, v1, 0x7362);
+                                a[r][0] = codes_f16<0x4140>(p01);
+                                a[r][1] = codes_f16<0x4342>(p01);
+                                a[r][2] = codes_f16<0x4140>(p23);
+                                a[r][3] = codes_f16<0x4342>(p23);
+                            }
                         }
-                    } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t v0 = v[r & 1][(r >> 1) * 2][w] ^ 0x80808080u;
-                            const uint32_t v1 = v[r & 1][(r >> 1) * 2 + 1][w] ^ 0x80808080u;
-                            const uint32_t p01 = __byte_perm(v0, v1, 0x5140), p23 = __byte_perm(v0, v1, 0x7362);
-                            a[r][0] = codes_f16<0x4140>(p01);
-                            a[r][1] = codes_f16<0x4342>(p01);
-                            a[r][2] = codes_f16<0x4140>(p23);
-                            a[r][3] = codes_f16<0x4342>(p23);
-                        }
-                    }
+                        for (int i = 0; i < (I8 ? 4 : 2); ++i) {
+                            const int k = z * S::kPerPiece + w * (I8 ? 4 : 2) + i;
 #pragma unroll
-                    for (int i = 0; i < (I8 ? 4 : 2); ++i) {
-                        const int k = z * S::kPerPiece + w * (I8 ? 4 : 2) + i;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma<BF>(acc[nt][k], a[0][i], a[1][i], a[2][i], a[3][i], hi0[nt], hi1[nt]);
-                            mma<BF>(acc[nt][k], a[0][i], a[1][i], a[2][i], a[3][i], lo0[nt], lo1[nt]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma<BF>(acc[nt][k], a[0][i], a[1][i], a[2][i], a[3][i], hi0[nt][m], hi1[nt][m]);
+                                mma<BF>(acc[nt][k], a[0][i], a[1][i], a[2][i], a[3][i], lo0[nt][m], lo1[nt][m]);
+                            }
                         }
                     }
                 }
-            }
             fetch(2 * j + S::kStages, wr);
             rd = rd + 1 == S::kStages ? 0 : rd + 1;
             wr = wr + 1 == S::kStages ? 0 : wr + 1;
@@ -565,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 if (g == 0) {
-                    s_m[warp * S::kHeads + head] = m[nt][e];
+                    s_m[warp * S::kHeads + head] = m_run[nt][e];
                     s_l[warp * S::kHeads + head] = sum;
                 }
                 float* dst = s_acc + (warp * S::kHeads + head) * (D + 4);
