@@ -63,6 +63,9 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int ha
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(have), "n"(N) : "memory");
 }
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -283,7 +286,18 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
         uint32_t bad = 0;                                 // those (mod 32) without a usable page
         size_t rows[kSubs];                               // cache rows of the step being fetched
         int have[kSubs];                                  // and its tokens, by 16
+        bool full = false;                                // whether all of them are there
         auto fetch_rows = [&](uint32_t dst, const uint8_t* cache) {
+            if (full) {
+#pragma unroll
+                for (int x = 0; x < S::kHalf / 512; ++x) {
+                    constexpr int kRows = 512 / S::kRow;
+                    const int m = x * kRows / 16;
+                    copy_async(dst + place<S::kRow>(x * kRows + lane / (S::kRow / 16), lane % (S::kRow / 16) * 16),
+                               cache + rows[m] * S::kRow + (x * 512 - m * 16 * S::kRow) + lane * 16);
+                }
+                return;
+            }
 #pragma unroll
             for (int x = 0; x < S::kHalf / 512; ++x) {
                 constexpr int kRows = 512 / S::kRow;      // rows per instruction, of one 16
@@ -304,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                         const int tok = t0 + kTile * (warp + kWarps * (j + lane / kSubs)) + lane % kSubs * 16;
                         ids = tok < t1 ? pages[tok >> p.log_page] : -1;
                     }
+                    full = t1 - t0 - kTile * (warp + kWarps * j) >= kTile;
 #pragma unroll
                     for (int m = 0; m < kSubs; ++m) {
                         const int at = (j * kSubs + m) & 31;
@@ -311,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                         const int tok = t0 + kTile * (warp + kWarps * j) + 16 * m;
                         const bool ok = page >= 0 && page < p.n_pages;
                         bad = (bad & ~(1u << at)) | (ok ? 0u : 1u << at);
+                        full = full && ok;
                         have[m] = ok ? min(16, t1 - tok) : 0;
                         rows[m] = (((ok ? static_cast<size_t>(page) : 0) * p.H + h) << p.log_page) +
                                   (tok & ((1 << p.log_page) - 1));
