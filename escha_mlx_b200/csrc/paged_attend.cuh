@@ -153,12 +153,21 @@ struct Shape {
     static constexpr int kHeads = 8 * NT;
     static constexpr int kFixed = (kAttendMaxBatch + 4) * 4 + 2 * kWarps * kHeads * 4 + kHeads * 4 + 64;
     // depth of a warp's ring: what the CTAs that share an SM leave
-    static constexpr int kMost = (226 * 1024 / kResident - 1024 - kFixed - kQBytes) / (kWarps * kRingStage);
+    static constexpr int kJoin = kWarps * kHeads * (D + 4) * 4;   // the warps' sums
+    static constexpr bool kAhead = kJoin - kWarps * kRingStage <= 2048;
+    static constexpr int kMost = (226 * 1024 / kResident - 1024 - kFixed - kQBytes - (kAhead ? 2048 : 0)) /
+                                 (kWarps * kRingStage);
     static constexpr int kStages = kMost > 8 ? 8 : kMost;
     static_assert(kStages >= 3, "a step's keys and values in flight beside what is in use");
-    static constexpr int kRing = kWarps * kStages * kRingStage;
-    static constexpr int kJoin = kWarps * kHeads * (D + 4) * 4;   // the warps' sums, over the ring
-    static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
+    // The warps' sums lie over the ring's stage 0 (with a little room behind it), so that a
+    // segment's first tiles can be fetched into the other stages before the one before it is
+    // joined; over the whole ring where they are much larger.
+    static constexpr int kAll = kWarps * kRingStage;      // a stage of all warps
+    static constexpr int kGap = kJoin > kAll ? kJoin - kAll : 0;
+    static constexpr int kRing = kStages * kAll;
+    static constexpr int kBody = kAhead ? kRing + kGap : kRing > kJoin ? kRing : kJoin;
+    static constexpr int kFirst = kAhead ? 1 : 0;
+    static __device__ constexpr int stage_at(int stage) { return stage * kAll + (kAhead && stage ? kGap : 0); }
     static constexpr int kShared = kBody + kQBytes + kFixed;
 };
 
@@ -240,53 +249,64 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
     }
     int unfinished_row = -1, unfinished_last = -1;
 
-    const uint32_t ring = smem_u32(s_body) + warp * (S::kStages * S::kRingStage);
-    const uint8_t* ring_ptr = s_body + warp * (S::kStages * S::kRingStage);
+    const uint32_t ring = smem_u32(s_body) + warp * S::kRingStage;
+    const uint8_t* ring_ptr = s_body + warp * S::kRingStage;
     const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache);
     const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
 
-    while (u < u_end) {
-        int b, rr, k0, k1, blocks, len;                   // rr: head and chunk
+    // A segment: blocks [k0, k1) of a row (rr: its head and chunk) of request b.
+    struct Segment { int b, rr, k0, k1, blocks; };
+    auto segment_at = [&](long long u) {
+        Segment x;
         if constexpr (CL) {
             const int row = c / p.ctas, part = c - row * p.ctas;
-            b = row / per_request;
-            rr = row - b * per_request;
-            len = min(max(p.lengths[b], 0), p.W << p.log_page);
-            blocks = (len + kAttendBlock - 1) / kAttendBlock;
-            k0 = blocks * part / p.ctas;
-            k1 = blocks * (part + 1) / p.ctas;
+            x.b = row / per_request;
+            x.rr = row - x.b * per_request;
+            x.blocks = (min(max(p.lengths[x.b], 0), p.W << p.log_page) + kAttendBlock - 1) / kAttendBlock;
+            x.k0 = x.blocks * part / p.ctas;
+            x.k1 = x.blocks * (part + 1) / p.ctas;
         } else {
             // the row that holds block u
             int hi = p.B;
-            b = 0;
-            while (hi - b > 1) {
-                const int mid = (b + hi) >> 1;
-                if (static_cast<long long>(s_prefix[mid]) * per_request <= u) b = mid; else hi = mid;
+            x.b = 0;
+            while (hi - x.b > 1) {
+                const int mid = (x.b + hi) >> 1;
+                if (static_cast<long long>(s_prefix[mid]) * per_request <= u) x.b = mid; else hi = mid;
             }
-            blocks = s_prefix[b + 1] - s_prefix[b];
-            const int in_request = static_cast<int>(u - static_cast<long long>(s_prefix[b]) * per_request);
-            rr = in_request / blocks;
-            k0 = in_request - rr * blocks;
-            k1 = static_cast<int>(min(static_cast<long long>(blocks), k0 + (u_end - u)));
-            len = min(max(p.lengths[b], 0), p.W << p.log_page);
+            x.blocks = s_prefix[x.b + 1] - s_prefix[x.b];
+            const int in_request = static_cast<int>(u - static_cast<long long>(s_prefix[x.b]) * per_request);
+            x.rr = in_request / x.blocks;
+            x.k0 = in_request - x.rr * x.blocks;
+            x.k1 = static_cast<int>(min(static_cast<long long>(x.blocks), x.k0 + (u_end - u)));
         }
-        const int h = rr / p.chunks, chunk = rr - h * p.chunks;
-        const int head0 = h * p.group + chunk * S::kHeads;
-        const int nheads = min(S::kHeads, p.group - chunk * S::kHeads);
-        const int t0 = k0 * kAttendBlock, t1 = min(len, k1 * kAttendBlock);
-        const bool starts = k0 == 0, ends = k1 == blocks;
-        const int32_t* pages = p.table + static_cast<size_t>(b) * p.W;
-
-        // tiles of this warp: warp, warp + kWarps, ... of the segment
-        constexpr int kSubs = S::kSubs, kTile = S::kTile;
-        const int tiles = (t1 - t0 + kTile - 1) / kTile;
-        const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-        const int halves = 2 * mine;                      // K0, V0, K1, V1, ...
-        int ids = -1;                                     // lane j: page of the 16 tokens j (mod 32)
-        uint32_t bad = 0;                                 // those (mod 32) without a usable page
-        size_t rows[kSubs];                               // cache rows of the step being fetched
-        int have[kSubs];                                  // and its tokens, by 16
-        bool full = false;                                // whether all of them are there
+        return x;
+    };
+    constexpr int kSubs = S::kSubs, kTile = S::kTile;
+    Segment seg;
+    int h, head0, nheads, t0, t1;                         // of the segment: heads and tokens
+    int mine, halves;                                     // this warp's steps warp, warp + kWarps, ...
+    const int32_t* pages;
+    int ids;                                              // lane j: page of the 16 tokens j (mod 32)
+    uint32_t bad;                                         // those (mod 32) without a usable page
+    size_t rows[kSubs];                                   // cache rows of the step being fetched
+    int have[kSubs];                                      // and its tokens, by 16
+    bool full = false;                                    // whether all of them are there
+    auto open = [&](const Segment& x) {
+        seg = x;
+        const int len = min(max(p.lengths[x.b], 0), p.W << p.log_page);
+        h = x.rr / p.chunks;
+        const int chunk = x.rr - h * p.chunks;
+        head0 = h * p.group + chunk * S::kHeads;
+        nheads = min(S::kHeads, p.group - chunk * S::kHeads);
+        t0 = x.k0 * kAttendBlock;
+        t1 = min(len, x.k1 * kAttendBlock);
+        const int steps = (t1 - t0 + kTile - 1) / kTile;
+        mine = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
+        halves = 2 * mine;                                // K0, V0, K1, V1, ...
+        pages = p.table + static_cast<size_t>(x.b) * p.W;
+        ids = -1;
+        bad = 0;
+    };
         auto fetch_rows = [&](uint32_t dst, const uint8_t* cache) {
             if (full) {
 #pragma unroll
@@ -312,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
         auto fetch = [&](int i, int stage) {
             if (i < halves) {
                 const int j = i >> 1;
-                const uint32_t dst = ring + stage * S::kRingStage;
+                const uint32_t dst = ring + S::stage_at(stage);
                 if ((i & 1) == 0) {
                     if ((j * kSubs & 31) == 0) {
                         const int tok = t0 + kTile * (warp + kWarps * (j + lane / kSubs)) + lane % kSubs * 16;
@@ -345,14 +365,17 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             }
             cp_async_commit();
         };
-        __syncthreads();      // the previous row's sums (in the ring) and queries are read
+        // the first kStages - 1 tiles of a segment, from stage kFirst on
+        auto prologue = [&]() {
+            __syncwarp();                                 // the other lanes' last reads
 #pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) fetch(i, i);
-
-        // queries of the row: lane (g, t) of chunk x holds head g's channels that meet the
+            for (int i = 0; i < S::kStages - 1; ++i) fetch(i, (S::kFirst + i) % S::kStages);
+        };
+        // queries of the segment: lane (g, t) of chunk x holds head g's channels that meet the
         // lane's bytes of the key rows
-        if (warp < NT) {
-            const int nt = warp;
+        auto load_queries = [&]() {
+            if (warp >= NT) return;
+            const int nt = warp, b = seg.b;
             const bool in = nt * 8 + g < nheads;
             const QT* src = q + static_cast<long>(b) * p.q_row +
                             static_cast<long>(head0 + (in ? nt * 8 + g : 0)) * p.q_head;
@@ -394,8 +417,16 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
 #pragma unroll
             for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
                 reinterpret_cast<uint4*>(s_q)[(nt * (S::kChunks * S::kQWords / 4) + x) * 32 + lane] = w[x];
-        }
+        };
+
+    bool more = u < u_end;
+    if (more) {
+        open(segment_at(u));
+        prologue();
+        load_queries();
         __syncthreads();
+    }
+    while (more) {
         float qs[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -415,12 +446,12 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             l[nt][0] = l[nt][1] = 0.0f;
         }
 
-        int rd = 0, wr = S::kStages - 1;                  // stages to read and to fill next
+        int rd = S::kFirst, wr = (S::kFirst + S::kStages - 1) % S::kStages;   // stages to read and to fill next
         for (int j = 0; j < mine; ++j) {
             // ---- scores of the step's tokens
             cp_async_wait<S::kStages - 2>();
             __syncwarp();         // the other lanes' copies; their reads of the stage to fill next
-            const uint8_t* tile = ring_ptr + rd * S::kRingStage;
+            const uint8_t* tile = ring_ptr + S::stage_at(rd);
             // two chains of products where the step has one tile only
             constexpr int kChains = kSubs == 1 ? 2 : 1;
             float s[NT][kSubs][kChains][4];
@@ -552,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             // ---- weighted values
             cp_async_wait<S::kStages - 2>();
             __syncwarp();
-            tile = ring_ptr + rd * S::kRingStage;
+            tile = ring_ptr + S::stage_at(rd);
 #pragma unroll
             for (int m = 0; m < kSubs; ++m)
 #pragma unroll
@@ -599,8 +630,18 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
         }
 
         // ---- join the warps through shared memory
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();                                  // every warp is through with its ring
+        const Segment was = seg;
+        const int was_head0 = head0, was_nheads = nheads;
+        const bool starts = was.k0 == 0, ends = was.k1 == was.blocks;
+        u += was.k1 - was.k0;
+        more = !CL && u < u_end;
+        if (more) {
+            // the next segment's first tiles are on their way meanwhile: the sums take the place
+            // of stage 0 only, which it uses last
+            open(segment_at(u));
+            if constexpr (S::kAhead) prologue();
+        }
+        __syncthreads();                                  // every warp is through with its stages
         float* s_acc = reinterpret_cast<float*>(s_body);  // [warp][head][D + 4]
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -627,9 +668,10 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                                             acc[nt][z * S::kPerPiece + k + 2][2 * half + e],
                                             acc[nt][z * S::kPerPiece + k + 3][2 * half + e]);
             }
+        if (more) load_queries();
         __syncthreads();
         const int slot = starts ? 2 * c + 1 : 2 * c;      // piece of an unfinished row
-        for (int i = tid; i < nheads * (D / 4); i += kThreads) {
+        for (int i = tid; i < was_nheads * (D / 4); i += kThreads) {
             const int head = i / (D / 4), d = (i % (D / 4)) * 4;
             float top = s_m[head];
 #pragma unroll
@@ -657,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             } else if (CL || (starts && ends)) {
                 // nothing to attend to (no usable page): zeros
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                QT* dst = out + (static_cast<size_t>(b) * heads_total + head0 + head) * D + d;
+                QT* dst = out + (static_cast<size_t>(was.b) * heads_total + was_head0 + head) * D + d;
                 *reinterpret_cast<uint2*>(dst) =
                     make_uint2(pack2<QBF>(o.x * inv, o.y * inv), pack2<QBF>(o.z * inv, o.w * inv));
             } else {
@@ -670,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             if (p.ctas > 1) {
                 cg::cluster_group cluster = cg::this_cluster();
                 cluster.sync();
-                const int items = nheads * (D / 4);
+                const int items = was_nheads * (D / 4);
                 for (int i = cluster.block_rank() * kThreads + tid; i < items; i += p.ctas * kThreads) {
                     const int head = i / (D / 4), d = (i % (D / 4)) * 4;
                     float2 ml[kMaxCluster];
@@ -699,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                             o.w += a * x[r].w;
                         }
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    QT* dst = out + (static_cast<size_t>(b) * heads_total + head0 + head) * D + d;
+                    QT* dst = out + (static_cast<size_t>(was.b) * heads_total + was_head0 + head) * D + d;
                     *reinterpret_cast<uint2*>(dst) =
                         make_uint2(pack2<QBF>(o.x * inv, o.y * inv), pack2<QBF>(o.z * inv, o.w * inv));
                 }
@@ -708,16 +750,19 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             return;
         }
         if (starts && !ends) {
-            unfinished_row = b * per_request + rr;
+            unfinished_row = was.b * per_request + was.rr;
             // last CTA of the row: the one whose share holds the row's last block
-            const long long last = static_cast<long long>(s_prefix[b]) * per_request +
-                                   static_cast<long long>(rr + 1) * blocks - 1;
+            const long long last = static_cast<long long>(s_prefix[was.b]) * per_request +
+                                   static_cast<long long>(was.rr + 1) * was.blocks - 1;
             long long cl = last * shares / total;         // near; settled by the shares themselves
             while (cl + 1 < shares && total * (cl + 1) / shares <= last) ++cl;
             while (cl > 0 && total * cl / shares > last) --cl;
             unfinished_last = static_cast<int>(cl);
         }
-        u += k1 - k0;
+        if (more) {
+            __syncthreads();                              // the sums are read
+            if constexpr (!S::kAhead) prologue();
+        }
     }
     if (tid == 0 && p.meta != nullptr) {
         p.meta[2 * c] = unfinished_row;
