@@ -1049,7 +1049,7 @@ int escha_paged_attend(const void* q, long q_row, long q_head, int q_type, const
     const int each = B < escha::kAttendMaxBatch ? B : escha::kAttendMaxBatch;
     const int sms = device_sms();
     const escha::AttendShape s = escha::attend_shape(each, H, group, D, W, lp, sms);
-    REQUIRE(((static_cast<long long>(W) << lp) / escha::kAttendBlock + 1) * each * H * s.chunks <
+    REQUIRE(((static_cast<long long>(W) << lp) / escha::kAttendBlock + 8) * each * H * s.chunks <
                 0x7fffffffll,
             "%s: %d requests of up to %lld tokens and %d heads are more than one launch numbers",
             __func__, each, static_cast<long long>(W) << lp, H);
@@ -1068,6 +1068,7 @@ int escha_paged_attend(const void* q, long q_row, long q_head, int q_type, const
     p.scale_log2 = scale * 1.4426950408889634f;
     p.H = H; p.group = group; p.chunks = s.chunks; p.heads = s.heads; p.D = D; p.W = W;
     p.log_page = lp; p.n_pages = n_pages;
+    p.row_cost = escha::attend_row_cost(D * (cache_type == ESCHA_I8 ? 1 : 2));
     // larger batches take one launch after the other (each waits for the one before, so they
     // share the workspace; a smaller last one needs no more of it)
     for (int b = 0; b < B; b += each) {

@@ -65,6 +65,7 @@ struct AttendParams {
     float* part;             // [2 * ctas][heads][D]
     float scale_log2;        // score scale times log2(e)
     int B, H, group, chunks, heads, D, W, log_page, n_pages, ctas;
+    int row_cost;            // blocks that the start of a row counts for
 };
 // How rows (a request's query heads of one key/value head) are shared out: a cluster each,
 // equal shares that cut rows (and a join), or equal shares that cannot.
@@ -76,6 +77,8 @@ struct AttendShape {
     int ctas;     // CTAs per row (cluster), or of the launch
     size_t meta_bytes, ml_bytes, part_bytes;
 };
+// What starting a row costs, in blocks of its cache (a row of `bytes` per token).
+constexpr int attend_row_cost(int bytes) { return (384 + bytes / 2) / bytes; }
 AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, int sms);
 cudaError_t launch_attend(const AttendParams& p, int q_type, int cache_type, AttendForm form,
                           cudaStream_t st);

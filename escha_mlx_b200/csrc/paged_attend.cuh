@@ -28,7 +28,8 @@
 //
 // Split.  The work is a line of blocks of 64 tokens, over all requests and key/value heads;
 // each CTA takes an equal share of it, whatever the lengths are, and cuts rows where its share
-// ends.  A CTA leaves at most two unfinished rows (its first and its last); a second, chained
+// ends.  Every row counts for some blocks more than it has (the exchange between its warps and
+// its first loads), so that a CTA with many short rows is not the last.  A CTA leaves at most two unfinished rows (its first and its last); a second, chained
 // kernel joins the pieces of each row in order.  No counters, nothing to clear.  Where all rows
 // fit the GPU at once and none can be long, a row is cut between the CTAs of a cluster instead,
 // which join through distributed shared memory: one launch and no scratch.
@@ -171,7 +172,7 @@ struct Shape {
     static constexpr int kShared = kBody + kQBytes + kFixed;
 };
 
-// Exclusive prefix of the requests' block counts in s_prefix[0 .. B], by the whole CTA.
+// Exclusive prefix of the requests' blocks and row costs in s_prefix[0 .. B], by the whole CTA.
 __device__ __forceinline__ void block_counts(const AttendParams& p, int* s_prefix, int* s_sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kEach = kAttendMaxBatch / kThreads;
@@ -181,7 +182,7 @@ __device__ __forceinline__ void block_counts(const AttendParams& p, int* s_prefi
     for (int i = 0; i < kEach; ++i) {
         const int b = tid * kEach + i;
         const int len = b < p.B ? min(max(p.lengths[b], 0), most) : 0;
-        n[i] = (len + kAttendBlock - 1) / kAttendBlock;
+        n[i] = len > 0 ? (len + kAttendBlock - 1) / kAttendBlock + p.row_cost : 0;
         sum += n[i];
     }
     int inc = sum;
@@ -255,7 +256,8 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
     const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
 
     // A segment: blocks [k0, k1) of a row (rr: its head and chunk) of request b.
-    struct Segment { int b, rr, k0, k1, blocks; };
+    // used: what of the line it takes up.
+    struct Segment { int b, rr, k0, k1, blocks, used; };
     auto segment_at = [&](long long u) {
         Segment x;
         if constexpr (CL) {
@@ -265,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             x.blocks = (min(max(p.lengths[x.b], 0), p.W << p.log_page) + kAttendBlock - 1) / kAttendBlock;
             x.k0 = x.blocks * part / p.ctas;
             x.k1 = x.blocks * (part + 1) / p.ctas;
+            x.used = 1;
         } else {
             // the row that holds block u
             int hi = p.B;
@@ -273,11 +276,14 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                 const int mid = (x.b + hi) >> 1;
                 if (static_cast<long long>(s_prefix[mid]) * per_request <= u) x.b = mid; else hi = mid;
             }
-            x.blocks = s_prefix[x.b + 1] - s_prefix[x.b];
+            const int units = s_prefix[x.b + 1] - s_prefix[x.b];      // the row's cost, then its blocks
             const int in_request = static_cast<int>(u - static_cast<long long>(s_prefix[x.b]) * per_request);
-            x.rr = in_request / x.blocks;
-            x.k0 = in_request - x.rr * x.blocks;
-            x.k1 = static_cast<int>(min(static_cast<long long>(x.blocks), x.k0 + (u_end - u)));
+            x.rr = in_request / units;
+            const int at = in_request - x.rr * units;
+            x.used = static_cast<int>(min(static_cast<long long>(units - at), u_end - u));
+            x.blocks = units - p.row_cost;
+            x.k0 = max(at - p.row_cost, 0);
+            x.k1 = max(at + x.used - p.row_cost, 0);
         }
         return x;
     };
@@ -419,9 +425,20 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                 reinterpret_cast<uint4*>(s_q)[(nt * (S::kChunks * S::kQWords / 4) + x) * 32 + lane] = w[x];
         };
 
-    bool more = u < u_end;
+    // the next segment with a block in it (a share may end within the cost of a row)
+    auto next = [&]() {
+        while (u < u_end) {
+            const Segment x = segment_at(u);
+            u += x.used;
+            if (CL || x.k1 > x.k0) {
+                open(x);
+                return true;
+            }
+        }
+        return false;
+    };
+    bool more = next();
     if (more) {
-        open(segment_at(u));
         prologue();
         load_queries();
         __syncthreads();
@@ -633,13 +650,11 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
         const Segment was = seg;
         const int was_head0 = head0, was_nheads = nheads;
         const bool starts = was.k0 == 0, ends = was.k1 == was.blocks;
-        u += was.k1 - was.k0;
-        more = !CL && u < u_end;
-        if (more) {
+        more = next();
+        if constexpr (S::kAhead) {
             // the next segment's first tiles are on their way meanwhile: the sums take the place
             // of stage 0 only, which it uses last
-            open(segment_at(u));
-            if constexpr (S::kAhead) prologue();
+            if (more) prologue();
         }
         __syncthreads();                                  // every warp is through with its stages
         float* s_acc = reinterpret_cast<float*>(s_body);  // [warp][head][D + 4]
@@ -753,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             unfinished_row = was.b * per_request + was.rr;
             // last CTA of the row: the one whose share holds the row's last block
             const long long last = static_cast<long long>(s_prefix[was.b]) * per_request +
-                                   static_cast<long long>(was.rr + 1) * was.blocks - 1;
+                                   static_cast<long long>(was.rr + 1) * (was.blocks + p.row_cost) - 1;
             long long cl = last * shares / total;         // near; settled by the shares themselves
             while (cl + 1 < shares && total * (cl + 1) / shares <= last) ++cl;
             while (cl > 0 && total * cl / shares > last) --cl;
