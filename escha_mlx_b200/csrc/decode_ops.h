@@ -77,8 +77,11 @@ struct AttendShape {
     int ctas;     // CTAs per row (cluster), or of the launch
     size_t meta_bytes, ml_bytes, part_bytes;
 };
-// What starting a row costs, in blocks of its cache (a row of `bytes` per token).
-constexpr int attend_row_cost(int bytes) { return (384 + bytes / 2) / bytes; }
+// What starting a row costs, in blocks of its cache (`bytes` per token).  Measured with 32 to 64
+// ragged requests, cost 0 / 2 / 4 / 8 / 16: 512 bytes 57.8 / 54.3 / 54.4 / 54.3 / 53.7 us, 256
+// bytes 87.8 / 69.4 / 69.0 / 68.8 / 69.9, 128 bytes 110 / 99 / 88 / 80 / 83, 64 bytes 117 / 108 /
+// 100 / 92 / 94.
+constexpr int attend_row_cost(int bytes) { return 1024 / bytes < 8 ? 1024 / bytes : 8; }
 AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, int sms);
 cudaError_t launch_attend(const AttendParams& p, int q_type, int cache_type, AttendForm form,
                           cudaStream_t st);
