@@ -97,6 +97,23 @@ def _load() -> ctypes.CDLL:
 lib = _load()
 
 
+def _load_decode():
+    """The binding of the decode step's operators (csrc/bind.cpp), over this library."""
+    try:
+        from . import _decode
+    except ImportError as exc:
+        raise ImportError(
+            f"escha_mlx_b200/_decode.so is missing or does not fit this torch ({exc}): build it with "
+            "`python -m escha_mlx_b200.csrc.build`. This package has no fallback.") from exc
+    _decode.init(*[ctypes.cast(getattr(lib, name), _vp).value for name in (
+        "escha_last_error", "escha_page_plan", "escha_paged_append",
+        "escha_paged_attend_workspace_bytes", "escha_paged_attend", "escha_sample")])
+    return _decode
+
+
+decode = _load_decode()
+
+
 def check(rc: int) -> None:
     if rc == ESCHA_OK:
         return
