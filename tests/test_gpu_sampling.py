@@ -218,3 +218,21 @@ def test_refusals(cuda):
         with pytest.raises(ValueError, match=text):
             sampling.sample(*bad)
     assert sampling.sample(x[:0], u[:0]).shape == (0,)
+
+
+def test_a_nucleus_that_the_counts_misplace(cuda):
+    """Half of the weight in tokens equal to the largest (at the top of their bin), the other
+    half thinly spread at the bottom of theirs: the bins' counts put the cut far from where it
+    is, and the exact weights of all bins have to find it."""
+    per_nat = 1023 / 30.25                     # bins of (max x - x) / T per unit
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    b = torch.randint(30, 330, (100000,), device=cuda, generator=gen).double()
+    x = -(b + 0.995) / per_nat
+    n = int(torch.exp(x).sum().item())
+    x = torch.cat([torch.zeros(n, device=cuda, dtype=torch.float64), x])
+    x = x[torch.randperm(len(x), device=cuda, generator=gen)].float().repeat(3, 1)
+    u = torch.tensor([0.1, 0.7, 0.999], device=cuda)
+    for p in (0.55, 0.6, 0.75, 0.95):
+        for m in (0.0, 0.01):
+            check(sampling.sample(x, u, 1.0, 0, p, m), x, u, 1.0, 0, p, m)
+            check(sampling.sample(x, u, 1.0, 90000, p, m), x, u, 1.0, 90000, p, m)
