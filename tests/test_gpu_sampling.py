@@ -221,18 +221,17 @@ def test_refusals(cuda):
 
 
 def test_a_nucleus_that_the_counts_misplace(cuda):
-    """Half of the weight in tokens equal to the largest (at the top of their bin), the other
-    half thinly spread at the bottom of theirs: the bins' counts put the cut far from where it
-    is, and the exact weights of all bins have to find it."""
+    """Three quarters of the weight in tokens equal to the largest (at the top of their bin), the
+    rest thinly spread at the bottom of the others: the bins' counts put a cut behind the first
+    several bins from where it is, and the exact weights of all bins have to find it."""
     per_nat = 1023 / 30.25                     # bins of (max x - x) / T per unit
-    gen = torch.Generator(device=cuda).manual_seed(0)
-    b = torch.randint(30, 330, (100000,), device=cuda, generator=gen).double()
-    x = -(b + 0.995) / per_nat
-    n = int(torch.exp(x).sum().item())
-    x = torch.cat([torch.zeros(n, device=cuda, dtype=torch.float64), x])
-    x = x[torch.randperm(len(x), device=cuda, generator=gen)].float().repeat(3, 1)
+    spread = np.concatenate([np.full(round(1500 / 190 * np.exp((b + 0.995) / per_nat)), b)
+                             for b in range(30, 220)])
+    x = np.concatenate([np.zeros(4500), -(spread + 0.995) / per_nat])
+    x = np.random.default_rng(0).permutation(x)
+    x = torch.from_numpy(x).float().to(cuda).repeat(3, 1)
     u = torch.tensor([0.1, 0.7, 0.999], device=cuda)
-    for p in (0.55, 0.6, 0.75, 0.95):
+    for p in (0.76, 0.77, 0.8, 0.9):
         for m in (0.0, 0.01):
             check(sampling.sample(x, u, 1.0, 0, p, m), x, u, 1.0, 0, p, m)
-            check(sampling.sample(x, u, 1.0, 90000, p, m), x, u, 1.0, 90000, p, m)
+            check(sampling.sample(x, u, 1.0, 150000, p, m), x, u, 1.0, 150000, p, m)
