@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
             float by = p.scale_log2;
             if constexpr (I8 && QBF) {
                 // bfloat16 queries against codes in binary16: bring the row's largest value
-                // to [1, 2) by a power of two
+                // to [2^14, 2^15) by a power of two, so that small ones beside it keep their bits
                 float top = 0.0f;
 #pragma unroll
                 for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
@@ -407,8 +407,8 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 120);
-                const float down = __int_as_float((127 - e) << 23);
-                by *= __int_as_float((127 + e) << 23);
+                const float down = __int_as_float((127 + 14 - e) << 23);
+                by *= __int_as_float((127 - 14 + e) << 23);
 #pragma unroll
                 for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
                     uint32_t* v = &w[x].x;

@@ -491,9 +491,10 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
     weight.top = top;
     weight.inv512 = k512 / static_cast<double>(temperature);
     weight.pow2 = s.pow2;
-    // bins of (top - x) / T; finite, so that the top itself has bin 0 at any temperature
-    const float bins = fminf(kBinsPerNat / temperature, 3e38f);
-    auto place_of = [&](float x) { return (top - x) * bins; };
+    // bins of (top - x) / T; a finite factor, so that the top itself has bin 0 at any
+    // temperature, and half the difference, which does not overflow
+    const float bins = fminf(2.0f * kBinsPerNat / temperature, 3e38f), half_top = 0.5f * top;
+    auto place_of = [&](float x) { return fmaf(-0.5f, x, half_top) * bins; };
     auto bin_of = [&](float x) {
         const float z = place_of(x);
         return z < static_cast<float>(kBins - 1) ? static_cast<int>(z) : kBins - 1;
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
         int last = kBins - 1;
         if (p_on && !k_on)
             last = min(last, static_cast<int>((logf(static_cast<float>(p.V) / (1.0f - share)) + 1e-2f) * kBinsPerNat) + 1);
-        if (!k_on) last = min(last, m_bin + 1);
+        else if (!k_on) last = min(last, m_bin + 1);
         for (int v = tid; v < vecs; v += kThreads) {
             const uint4 q = xv[v];
             const T* e = reinterpret_cast<const T*>(&q);

@@ -304,6 +304,37 @@ def test_attend_large_batches(cuda, b):
     Case(cuda, rng.integers(0, 90, b), 1, 2, 64, 16, "f16", "f16").check()
 
 
+@pytest.mark.parametrize("lens", [[0, 0, 0], [0, 1, 5], [64, 0, 65, 0, 0, 3]])
+def test_attend_short_rows_of_wide_tables(cuda, lens):
+    """Fewer blocks of tokens than CTAs, or none, where rows may be cut."""
+    Case(cuda, lens, 2, 8, 128, 16, "f16", "f16", spare=400).check()
+
+
+@pytest.mark.parametrize("cache,kind", TYPES)
+@pytest.mark.parametrize("b,h", [(400, 1), (37, 2), (100, 1), (20, 8), (3, 99)])
+def test_attend_every_way_of_sharing_rows(cuda, cache, kind, b, h):
+    rng = np.random.default_rng(b)
+    Case(cuda, rng.integers(0, 65, b), h, 2, 64, 16, cache, kind, spare=0).check()     # one block
+    Case(cuda, rng.integers(0, 600, b), h, 2, 64, 16, cache, kind, spare=0).check()
+
+
+def test_attend_requests_that_share_pages(cuda):
+    c = Case(cuda, [200, 200, 64], 2, 4, 64, 16, "f16", "f16")
+    c.table[1] = c.table[0]
+    c.t = ints(c.table, cuda)
+    c.check()
+
+
+def test_attend_queries_of_one_large_channel(cuda):
+    """bfloat16 queries whose largest channel dwarfs the others and meets zeros in the cache:
+    the others decide the scores."""
+    c = Case(cuda, [300, 20], 2, 4, 64, 16, "int8", "bf16")
+    c.q[:, :, 5] = 2.0**18
+    c.cache.k[..., 5] = 0
+    c.values[0][..., 5] = 0
+    c.check()
+
+
 def test_attend_leaves_out_pages_that_do_not_exist(cuda):
     c = Case(cuda, [100, 40, 300, 16], 2, 4, 128, 16, "f16", "f16")
     c.table[0, 2], c.table[2, 0], c.table[2, 18] = -1, 10**6, -2**31

@@ -80,7 +80,7 @@ SETTINGS = [
     (0.8, 40, 0.95, 0.02), (1.3, 1, 0.5, 0.5), (0.0, 5, 0.5, 0.1), (1.5, 1000, 0.99, 0.0),
     (2.0, 3000, 0.999, 0.0), (3.0, 0, 0.97, 0.0), (3.0, 5000, 1.0, 0.0), (1.0, 0, 0.0, 0.0),
     (1.0, 0, 0.3, 1.0), (0.05, 10, 0.9, 0.0), (20.0, 0, 0.9, 0.0), (100.0, 20000, 0.6, 0.001),
-    (float("nan"), 3, 0.5, 0.1), (1e-30, 0, 0.9, 0.0), (1e30, 0, 0.9, 0.0), (1.0, -3, 2.0, -1.0),
+    (1.0, 0, 0.9, 0.05), (3.0, 0, 0.95, 0.3), (20.0, 0, 0.8, 0.5), (float("nan"), 3, 0.5, 0.1), (1e-30, 0, 0.9, 0.0), (1e30, 0, 0.9, 0.0), (1.0, -3, 2.0, -1.0),
 ]
 
 
@@ -124,6 +124,17 @@ def test_masked_and_unusual_logits(cuda, v):
     h = x.half()                                          # the lowest value becomes -inf
     for s in SETTINGS[:8]:
         check(sampling.sample(h, u, *s), h, u, *s)
+
+
+def test_logits_at_the_ends_of_their_type(cuda):
+    """Differences past the type's largest value, at temperatures that bring them back."""
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    x = 6.6e38 * (torch.rand((4, 30000), device=cuda, generator=gen, dtype=torch.float64) - 0.5)
+    x = x.float()
+    u = torch.rand((4,), device=cuda, generator=gen)
+    for s in ((1e38, 0, 1.0, 0.0), (1e38, 0, 0.7, 0.0), (5e37, 300, 1.0, 0.0), (1e37, 0, 0.9, 0.05),
+              (3e38, 9000, 0.9, 0.0), (1.0, 0, 0.9, 0.0)):
+        check(sampling.sample(x, u, *s), x, u, *s)
 
 
 def test_settings_by_row(cuda):
