@@ -166,14 +166,19 @@ template <> struct Pair<__nv_bfloat16> {
     }
 };
 
-// The code nearest to x / scale, ties to even.  The rounded quotient can land on the wrong
-// side of a middle; its remainder x - code * scale (one rounding, by FMA) tells.
-__device__ __forceinline__ int code_of(float x, float scale) {
-    float c = rintf(__fdiv_rn(x, scale));
-    const float r = __fmaf_rn(-c, scale, x), half = 0.5f * scale;
-    if (r > half) c += 1.0f;
-    else if (r < -half) c -= 1.0f;
-    return static_cast<int>(fminf(fmaxf(c, -127.0f), 127.0f));
+// The code nearest to x / scale, ties to even, from a guess that is off by one at most.  Whether
+// x lies above the middle between two codes is the sign of x - (c +- 1/2) scale, which one fused
+// multiply-add gives exactly (a rounded quotient can land on the wrong side); `times` 2 keeps
+// the half of a denormal scale.  Adding 1.5 * 2^23 rounds to an integer and leaves it in the low
+// bits.
+__device__ __forceinline__ uint32_t code_of(float x, float scale, float guess, float times) {
+    const float shifted = guess + 12582912.0f, c = shifted - 12582912.0f;
+    const int bits = __float_as_int(shifted);
+    const bool odd = bits & 1;
+    const float above = __fmaf_rn(-times * (c + 0.5f), scale, times * x);
+    const float below = __fmaf_rn(-times * (c - 0.5f), scale, times * x);
+    const int up = above > 0.0f || (odd && above == 0.0f), down = below < 0.0f || (odd && below == 0.0f);
+    return static_cast<uint32_t>(min(max(((bits << 8) >> 8) - 0x400000 + up - down, -127), 127)) & 0xffu;
 }
 
 constexpr int kAppendThreads = 256;
@@ -233,8 +238,7 @@ paged_append_kernel(const AppendParams p, int log_d8) {
             } else {
                 const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
                 float f[8];
-                float top = 0.0f;
-                bool odd = false;                         // NaN or infinite
+                float top = 0.0f, nothing = 0.0f;         // NaN if a value is not finite
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float2 y = Pair<T>::f32(w[k]);
@@ -244,20 +248,36 @@ paged_append_kernel(const AppendParams p, int log_d8) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     top = fmaxf(top, fabsf(f[k]));
-                    odd |= !(fabsf(f[k]) <= 3.4e38f);
+                    nothing = fmaf(f[k], 0.0f, nothing);
                 }
-                if (odd) top = __int_as_float(0x7f800000);
+                if (!(nothing == 0.0f)) top = __int_as_float(0x7f800000);
                 for (unsigned o = d8 >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 // a row that is not finite is stored as NaN: its values have no scale
                 const bool finite = top <= 3.4e38f;
                 const float scale = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fc00000);
                 if (slot[j] >= 0) {
                     uint32_t c[2] = {0, 0};
-                    if (finite && scale > 0.0f) {
+                    if (finite && scale > 1e-36f) {
+                        const float by = __frcp_rn(scale);
+                        float edge = 0.0f;                // how near to a middle the quotients come
+                        uint32_t b[8];
 #pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float t = f[k] * by, shifted = t + 12582912.0f;
+                            edge = fmaxf(edge, fabsf(t - (shifted - 12582912.0f)));
+                            b[k] = __float_as_uint(shifted);
+                        }
+                        // t is good to 2e-5: nearer than that, the exact comparison
+                        if (edge > 0.4999f)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) b[k] = code_of(f[k], scale, f[k] * by, 1.0f);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            c[k] = __byte_perm(__byte_perm(b[4 * k], b[4 * k + 1], 0x0040),
+                                               __byte_perm(b[4 * k + 2], b[4 * k + 3], 0x0040), 0x5410);
+                    } else if (finite && scale > 0.0f) {          // its reciprocal may not exist
                         for (int k = 0; k < 8; ++k)
-                            c[k >> 2] |= (static_cast<uint32_t>(code_of(f[k], scale)) & 0xffu)
-                                         << (8 * (k & 3));
+                            c[k >> 2] |= code_of(f[k], scale, __fdiv_rn(f[k], scale), 2.0f) << (8 * (k & 3));
                     }
                     int8_t* dst = static_cast<int8_t*>(is_v[j] ? p.v_cache : p.k_cache) + at * p.D + d * 8;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);

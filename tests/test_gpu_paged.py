@@ -160,6 +160,30 @@ def test_append_stores_rows_at_their_slots(cuda, cache, kind, t, h, d, page):
         assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_append_codes_at_every_magnitude(cuda, kind):
+    """Codes and scales equal the definition's from the smallest denormals to the largest values,
+    ties between codes among them."""
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    low, high = (-24, 15) if kind == "f16" else (-133, 127)
+    x = torch.randn((64 * 16, 2, 64), device=cuda, generator=gen, dtype=torch.float64)
+    x[::3] = torch.randint(-254, 255, x[::3].shape, device=cuda, generator=gen).double() / 2
+    x[::3, :, 0] = 127.0                                       # scale 1: halves are ties
+    by = torch.randint(low, high, (x.shape[0], 2, 1), device=cuda, generator=gen)
+    top = x.abs().amax(-1, keepdim=True)
+    x = torch.where(torch.arange(x.shape[0], device=cuda)[:, None, None] % 3 == 0,
+                    x * torch.exp2((by.clamp(max=high - 8)).double()), x / top * 1.98 * torch.exp2(by.double()))
+    x = x.to(DT[kind])
+    pc = paged.PagedCache(64, 16, 2, 64, torch.int8, cuda)
+    pc.append(x, x.flip(0), torch.arange(64 * 16, device=cuda, dtype=torch.int32))
+    for name, rows in (("k", x), ("v", x.flip(0))):
+        codes, scale = quantised(rows.double().cpu().numpy())
+        got = getattr(pc, name).cpu().numpy().transpose(0, 2, 1, 3).reshape(codes.shape)
+        got_scale = getattr(pc, name + "_scale").cpu().numpy().transpose(0, 2, 1).reshape(scale.shape)
+        assert np.array_equal(got_scale, scale)
+        assert np.array_equal(got, codes)
+
+
 def test_append_takes_any_stride_and_alignment(cuda):
     h, d, t = 2, 64, 9
     gen = torch.Generator(device=cuda).manual_seed(0)
