@@ -313,117 +313,117 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
         ids = -1;
         bad = 0;
     };
-        auto fetch_rows = [&](uint32_t dst, const uint8_t* cache) {
-            if (full) {
-#pragma unroll
-                for (int x = 0; x < S::kHalf / 512; ++x) {
-                    constexpr int kRows = 512 / S::kRow;
-                    const int m = x * kRows / 16;
-                    copy_async(dst + place<S::kRow>(x * kRows + lane / (S::kRow / 16), lane % (S::kRow / 16) * 16),
-                               cache + rows[m] * S::kRow + (x * 512 - m * 16 * S::kRow) + lane * 16);
-                }
-                return;
-            }
+    auto fetch_rows = [&](uint32_t dst, const uint8_t* cache) {
+        if (full) {
 #pragma unroll
             for (int x = 0; x < S::kHalf / 512; ++x) {
-                constexpr int kRows = 512 / S::kRow;      // rows per instruction, of one 16
+                constexpr int kRows = 512 / S::kRow;
                 const int m = x * kRows / 16;
-                const int r = x * kRows % 16 + lane / (S::kRow / 16);
-                const int byte = lane % (S::kRow / 16) * 16;
-                const bool in = r < have[m];
-                copy_async<16>(dst + place<S::kRow>(m * 16 + r, byte),
-                               cache + rows[m] * S::kRow + (in ? r * S::kRow + byte : 0), in ? 16 : 0);
+                copy_async(dst + place<S::kRow>(x * kRows + lane / (S::kRow / 16), lane % (S::kRow / 16) * 16),
+                           cache + rows[m] * S::kRow + (x * 512 - m * 16 * S::kRow) + lane * 16);
             }
-        };
-        auto fetch = [&](int i, int stage) {
-            if (i < halves) {
-                const int j = i >> 1;
-                const uint32_t dst = ring + S::stage_at(stage);
-                if ((i & 1) == 0) {
-                    if ((j * kSubs & 31) == 0) {
-                        const int tok = t0 + kTile * (warp + kWarps * (j + lane / kSubs)) + lane % kSubs * 16;
-                        ids = tok < t1 ? pages[tok >> p.log_page] : -1;
-                    }
-                    full = t1 - t0 - kTile * (warp + kWarps * j) >= kTile;
+            return;
+        }
 #pragma unroll
-                    for (int m = 0; m < kSubs; ++m) {
-                        const int at = (j * kSubs + m) & 31;
-                        const int page = __shfl_sync(0xffffffffu, ids, at);
-                        const int tok = t0 + kTile * (warp + kWarps * j) + 16 * m;
-                        const bool ok = page >= 0 && page < p.n_pages;
-                        bad = (bad & ~(1u << at)) | (ok ? 0u : 1u << at);
-                        full = full && ok;
-                        have[m] = ok ? min(16, t1 - tok) : 0;
-                        rows[m] = (((ok ? static_cast<size_t>(page) : 0) * p.H + h) << p.log_page) +
-                                  (tok & ((1 << p.log_page) - 1));
-                        if constexpr (I8) {
-                            // scales: lanes 0..15 K's, the others V's
-                            const float* src = (lane < 16 ? p.k_scale : p.v_scale) + rows[m];
-                            const bool in = (lane & 15) < have[m];
-                            copy_async<4>(dst + S::kHalf + (m * 32 + lane) * 4, src + (in ? lane & 15 : 0),
-                                          in ? 4 : 0);
-                        }
-                    }
-                    fetch_rows(dst, kc);
-                } else {
-                    fetch_rows(dst, vc);
+        for (int x = 0; x < S::kHalf / 512; ++x) {
+            constexpr int kRows = 512 / S::kRow;      // rows per instruction, of one 16
+            const int m = x * kRows / 16;
+            const int r = x * kRows % 16 + lane / (S::kRow / 16);
+            const int byte = lane % (S::kRow / 16) * 16;
+            const bool in = r < have[m];
+            copy_async<16>(dst + place<S::kRow>(m * 16 + r, byte),
+                           cache + rows[m] * S::kRow + (in ? r * S::kRow + byte : 0), in ? 16 : 0);
+        }
+    };
+    auto fetch = [&](int i, int stage) {
+        if (i < halves) {
+            const int j = i >> 1;
+            const uint32_t dst = ring + S::stage_at(stage);
+            if ((i & 1) == 0) {
+                if ((j * kSubs & 31) == 0) {
+                    const int tok = t0 + kTile * (warp + kWarps * (j + lane / kSubs)) + lane % kSubs * 16;
+                    ids = tok < t1 ? pages[tok >> p.log_page] : -1;
                 }
-            }
-            cp_async_commit();
-        };
-        // the first kStages - 1 tiles of a segment, from stage kFirst on
-        auto prologue = [&]() {
-            __syncwarp();                                 // the other lanes' last reads
+                full = t1 - t0 - kTile * (warp + kWarps * j) >= kTile;
 #pragma unroll
-            for (int i = 0; i < S::kStages - 1; ++i) fetch(i, (S::kFirst + i) % S::kStages);
-        };
-        // queries of the segment: lane (g, t) of chunk x holds head g's channels that meet the
-        // lane's bytes of the key rows
-        auto load_queries = [&]() {
-            if (warp >= NT) return;
-            const int nt = warp, b = seg.b;
-            const bool in = nt * 8 + g < nheads;
-            const QT* src = q + static_cast<long>(b) * p.q_row +
-                            static_cast<long>(head0 + (in ? nt * 8 + g : 0)) * p.q_head;
-            uint4 w[S::kChunks * S::kQWords / 4];
-#pragma unroll
-            for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
-                // 16 channels (8-bit cache) are two loads of 8
-                const int off = I8 ? (x >> 1) * 64 + t * 16 + (x & 1) * 8 : x * 32 + t * 8;
-                w[x] = in ? *reinterpret_cast<const uint4*>(src + off) : make_uint4(0, 0, 0, 0);
-            }
-            float by = p.scale_log2;
-            if constexpr (I8 && QBF) {
-                // bfloat16 queries against codes in binary16: bring the row's largest value
-                // to [2^14, 2^15) by a power of two, so that small ones beside it keep their bits
-                float top = 0.0f;
-#pragma unroll
-                for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 f = unpack2<true>(k == 0 ? w[x].x : k == 1 ? w[x].y : k == 2 ? w[x].z : w[x].w);
-                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 120);
-                const float down = __int_as_float((127 + 14 - e) << 23);
-                by *= __int_as_float((127 - 14 + e) << 23);
-#pragma unroll
-                for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
-                    uint32_t* v = &w[x].x;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 f = unpack2<true>(v[k]);
-                        v[k] = pack2<false>(f.x * down, f.y * down);
+                for (int m = 0; m < kSubs; ++m) {
+                    const int at = (j * kSubs + m) & 31;
+                    const int page = __shfl_sync(0xffffffffu, ids, at);
+                    const int tok = t0 + kTile * (warp + kWarps * j) + 16 * m;
+                    const bool ok = page >= 0 && page < p.n_pages;
+                    bad = (bad & ~(1u << at)) | (ok ? 0u : 1u << at);
+                    full = full && ok;
+                    have[m] = ok ? min(16, t1 - tok) : 0;
+                    rows[m] = (((ok ? static_cast<size_t>(page) : 0) * p.H + h) << p.log_page) +
+                              (tok & ((1 << p.log_page) - 1));
+                    if constexpr (I8) {
+                        // scales: lanes 0..15 K's, the others V's
+                        const float* src = (lane < 16 ? p.k_scale : p.v_scale) + rows[m];
+                        const bool in = (lane & 15) < have[m];
+                        copy_async<4>(dst + S::kHalf + (m * 32 + lane) * 4, src + (in ? lane & 15 : 0),
+                                      in ? 4 : 0);
                     }
                 }
+                fetch_rows(dst, kc);
+            } else {
+                fetch_rows(dst, vc);
             }
-            if (t == 0) s_qscale[nt * 8 + g] = by;
+        }
+        cp_async_commit();
+    };
+    // the first kStages - 1 tiles of a segment, from stage kFirst on
+    auto prologue = [&]() {
+        __syncwarp();                                 // the other lanes' last reads
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) fetch(i, (S::kFirst + i) % S::kStages);
+    };
+    // queries of the segment: lane (g, t) of chunk x holds head g's channels that meet the
+    // lane's bytes of the key rows
+    auto load_queries = [&]() {
+        if (warp >= NT) return;
+        const int nt = warp, b = seg.b;
+        const bool in = nt * 8 + g < nheads;
+        const QT* src = q + static_cast<long>(b) * p.q_row +
+                        static_cast<long>(head0 + (in ? nt * 8 + g : 0)) * p.q_head;
+        uint4 w[S::kChunks * S::kQWords / 4];
+#pragma unroll
+        for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
+            // 16 channels (8-bit cache) are two loads of 8
+            const int off = I8 ? (x >> 1) * 64 + t * 16 + (x & 1) * 8 : x * 32 + t * 8;
+            w[x] = in ? *reinterpret_cast<const uint4*>(src + off) : make_uint4(0, 0, 0, 0);
+        }
+        float by = p.scale_log2;
+        if constexpr (I8 && QBF) {
+            // bfloat16 queries against codes in binary16: bring the row's largest value
+            // to [2^14, 2^15) by a power of two, so that small ones beside it keep their bits
+            float top = 0.0f;
 #pragma unroll
             for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
-                reinterpret_cast<uint4*>(s_q)[(nt * (S::kChunks * S::kQWords / 4) + x) * 32 + lane] = w[x];
-        };
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = unpack2<true>(k == 0 ? w[x].x : k == 1 ? w[x].y : k == 2 ? w[x].z : w[x].w);
+                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 120);
+            const float down = __int_as_float((127 + 14 - e) << 23);
+            by *= __int_as_float((127 - 14 + e) << 23);
+#pragma unroll
+            for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x) {
+                uint32_t* v = &w[x].x;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = unpack2<true>(v[k]);
+                    v[k] = pack2<false>(f.x * down, f.y * down);
+                }
+            }
+        }
+        if (t == 0) s_qscale[nt * 8 + g] = by;
+#pragma unroll
+        for (int x = 0; x < S::kChunks * S::kQWords / 4; ++x)
+            reinterpret_cast<uint4*>(s_q)[(nt * (S::kChunks * S::kQWords / 4) + x) * 32 + lane] = w[x];
+    };
 
     // the next segment with a block in it (a share may end within the cost of a row)
     auto next = [&]() {
