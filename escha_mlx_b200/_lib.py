@@ -97,7 +97,7 @@ def _load() -> ctypes.CDLL:
 lib = _load()
 
 
-def _load_decode():
+def load_decode():
     """The binding of the decode step's operators (csrc/bind.cpp), over this library."""
     try:
         from . import _decode
@@ -109,9 +109,6 @@ def _load_decode():
         "escha_last_error", "escha_page_plan", "escha_paged_append",
         "escha_paged_attend_workspace_bytes", "escha_paged_attend", "escha_sample")])
     return _decode
-
-
-decode = _load_decode()
 
 
 def check(rc: int) -> None:

@@ -16,7 +16,9 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import decode
+from ._lib import load_decode
+
+decode = load_decode()
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.int8)
 HEAD_DIMS = (64, 128, 256)

@@ -8,7 +8,9 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import decode, lib
+from ._lib import lib, load_decode
+
+decode = load_decode()
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 

@@ -12,11 +12,16 @@ stream decodes with exactly the same instruction and byte counts as a trained on
 """
 from __future__ import annotations
 
+from typing import TYPE_CHECKING
+
 import numpy as np
 import torch
 
-from . import moe, paged, quant
+from . import moe, quant
 from .models.qwen3_5_moe import EschaSparseMoeBlock
+
+if TYPE_CHECKING:
+    from . import paged
 
 MOE_35B = dict(hidden=2048, inter=512, experts=256, top_k=8, K_gate_up=2, K_down=2,
                q_heads=16, kv_heads=2, head_dim=256)
@@ -96,6 +101,7 @@ class MoeLayer(torch.nn.Module):
 
     def new_cache(self, n_pages: int, page_size: int, dtype=torch.float16) -> paged.PagedCache:
         """An empty paged cache of this layer's key/value heads."""
+        from . import paged
         return paged.PagedCache(n_pages, page_size, self._kv_heads, self._head_dim, dtype,
                                 self.k._w8.device)
 
