@@ -99,6 +99,7 @@ struct SampleParams {
     int64_t* tokens;         // [B]
     long stride;
     int B, V, slice;
+    bool by_length;          // rows in the order of what their settings may cost
 };
 int sample_max_vocab(int type);
 cudaError_t launch_sample(const SampleParams& p, int type, cudaStream_t st);

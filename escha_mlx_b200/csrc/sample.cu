@@ -378,12 +378,29 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) sample_kernel(const Sample
     T* xs = reinterpret_cast<T*>(smem + sizeof(Shared));
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = cluster.block_rank(), ctas = cluster.num_blocks();
-    const int row = blockIdx.x / ctas;
+    int row = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_launch_dependents();
     s.pow2[tid] = exp2(tid / 512.0);
     if (tid == 0) s.list_n = 0;
     grid_dependency_wait();
+    if (p.by_length) {
+        // Rows that may keep most of the vocabulary take two to three times as long as those with
+        // a small top-k or none to draw: where rows wait for a place, the long ones go first.
+        int k = 0;
+        float t = 0.0f;
+        if (tid < p.B) {
+            t = p.temperature ? p.temperature[tid] : p.temperature1;
+            k = p.top_k ? p.top_k[tid] : p.top_k1;
+        }
+        const uint32_t is_long = tid < p.B && t > 0.0f && !(k > 0 && k <= kByMaxima);
+        uint32_t all;
+        const uint32_t upto = block_inclusive(is_long, s.scan32, &all);
+        const int place = is_long ? upto - 1 : all + (tid - upto);
+        if (tid < p.B && place == row) s.found = tid;
+        __syncthreads();
+        row = s.found;
+    }
 
     // settings of the row, on their way while the logits are read
     const float temperature = p.temperature ? p.temperature[row] : p.temperature1;
@@ -1101,8 +1118,13 @@ cudaError_t launch(const SampleParams& p, int ctas, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t launch(const SampleParams& p, int ctas, cudaStream_t st) {
-    return static_cast<long>(p.B) * ctas <= sm_count() ? launch<T, 1>(p, ctas, st) : launch<T, 2>(p, ctas, st);
+cudaError_t launch(SampleParams p, int ctas, cudaStream_t st) {
+    const long all = static_cast<long>(p.B) * ctas;
+    if (all <= sm_count()) return launch<T, 1>(p, ctas, st);
+    // with settings that differ, more CTAs than places, and a thread for each row to sort them
+    // (64 rows of 151936, mixed: 50 us against 54)
+    p.by_length = (p.temperature != nullptr || p.top_k != nullptr) && all > 2 * sm_count() && p.B <= kThreads;
+    return launch<T, 2>(p, ctas, st);
 }
 
 }  // namespace
