@@ -201,6 +201,19 @@ def test_append_takes_any_stride_and_alignment(cuda):
     pc.append(odd[:0], odd[:0], slots[:0])                         # nothing
 
 
+def test_append_more_rows_than_one_launch_numbers(cuda):
+    """70000 rows of 1024 heads of 256 (one row, repeated): three launches; almost all skipped."""
+    t, h, d = 70000, 1024, 256
+    x = torch.randn((1, h, d), device=cuda).half()
+    pc = paged.PagedCache(1, 16, h, d, torch.float16, cuda)
+    slots = torch.full((t,), -1, dtype=torch.int32, device=cuda)
+    at = [0, 32510, 32511, 32512, 32513, 65023, 65024, 69999]
+    slots[torch.tensor(at, device=cuda)] = torch.arange(8, dtype=torch.int32, device=cuda)
+    pc.append(x.expand(t, h, d), x.expand(t, h, d), slots)
+    for c in (pc.k, pc.v):
+        assert torch.equal(c[0, :, :8], x[0][:, None].expand(h, 8, d)) and not c[0, :, 8:].any()
+
+
 def test_rows_that_are_not_finite_are_stored_as_nan(cuda):
     for kind in (torch.float16, torch.bfloat16):
         x = torch.ones((4, 1, 64), device=cuda, dtype=kind)

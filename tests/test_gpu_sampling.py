@@ -151,6 +151,30 @@ def test_settings_by_row(cuda):
     check(got.view(-1), x, u, t, k, 0.9, m)
 
 
+def test_one_row_without_a_batch(cuda):
+    x, u = logits_of(cuda, 2, 3001, "f16", seed=9)
+    got = sampling.sample(x[1], u[1], 0.8, 50, 0.9)
+    assert got.shape == () and got.item() == sampling.sample(x, u, 0.8, 50, 0.9)[1].item()
+
+
+@pytest.mark.parametrize("b", [38, 511, 512, 513])
+def test_long_rows_first(cuda, b):
+    """More rows than the GPU holds at once, with settings of their own: every row's token is its
+    own whatever order they run in."""
+    v = 33000
+    x, u = logits_of(cuda, 4, v, "f16", seed=b)
+    x, u = x.repeat(-(-b // 4), 1)[:b], u.repeat(-(-b // 4))[:b]
+    pick = torch.randint(0, 4, (b,), device=cuda, generator=torch.Generator(device=cuda).manual_seed(b))
+    t = torch.tensor([0.0, 0.7, 1.0, 1.5], device=cuda)[pick]
+    k = torch.tensor([0, 40, 0, 2000], dtype=torch.int32, device=cuda)[pick]
+    got = sampling.sample(x, u, t, k, 0.95, 0.0)
+    for i in range(4):
+        one = sampling.sample(x[:4], u[:4], [0.0, 0.7, 1.0, 1.5][i], [0, 40, 0, 2000][i], 0.95, 0.0)
+        check(one, x[:4], u[:4], [0.0, 0.7, 1.0, 1.5][i], [0, 40, 0, 2000][i], 0.95, 0.0)
+        mine = (pick == i).nonzero()[:, 0]
+        assert torch.equal(got[mine], one[mine % 4])
+
+
 def test_uniforms_at_their_ends(cuda):
     x, _ = logits_of(cuda, 4, 9000, "f32", seed=3)
     u = torch.tensor([0.0, 2.0**-24, 1 - 2.0**-24, 0.5], device=cuda)
