@@ -18,6 +18,10 @@ extern template cudaError_t launch_any<true, true>(const AttendParams&, AttendFo
 // tokens 21 / 24 / 44 against 16 / 20 / 51.  With 37 requests (clusters of 4 that do not all fit
 // at once) 39 against 33 at 2048.
 constexpr int kClusterTokens = 2048;
+// The same for a few rows, with clusters of 16: 1 / 4 requests 9.4 / 13.6 us against 12.7 / 15.4
+// at 4096 tokens, 14.5 / 18.8 against 16.7 / 20.4 at 8192, 23 / 32 against 20 / 32 at 16384; 16
+// rows 28 against 20 at 4096 (not all at once either).
+constexpr int kWideTokens = 8192, kWideRows = 8;
 
 AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, int sms) {
     AttendShape s;
@@ -31,8 +35,11 @@ AttendShape attend_shape(int B, int H, int group, int D, int W, int log_page, in
         // a group), if they use most of the GPU or a row has no more blocks
         s.ctas = 1;
         while (s.ctas < 8 && s.ctas < blocks && 2 * s.ctas * rows <= fit - fit / 9) s.ctas *= 2;
-        if (rows <= fit && (s.ctas == 8 || s.ctas >= blocks || s.ctas * rows >= fit - fit / 2 + fit / 24))
+        if (rows <= fit && (s.ctas >= 8 || s.ctas >= blocks || s.ctas * rows >= fit - fit / 2 + fit / 24))
             s.form = kAttendCluster;
+    } else if (blocks * kAttendBlock <= kWideTokens && rows <= kWideRows) {
+        s.ctas = 16;
+        s.form = kAttendCluster;
     }
     if (s.form != kAttendCluster) {
         // rows are cut between blocks only

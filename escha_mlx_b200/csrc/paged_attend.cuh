@@ -54,7 +54,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxCluster = 8;
 
 // A lane's copy of N bytes, completed by cp.async.wait_group; bytes past `have` are zeros.
 template <int N>
@@ -730,31 +729,41 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
                 const int items = was_nheads * (D / 4);
                 for (int i = cluster.block_rank() * kThreads + tid; i < items; i += p.ctas * kThreads) {
                     const int head = i / (D / 4), d = (i % (D / 4)) * 4;
-                    float2 ml[kMaxCluster];
-                    float4 x[kMaxCluster];
-#pragma unroll
-                    for (int r = 0; r < kMaxCluster; ++r)
-                        if (r < p.ctas) {
-                            ml[r] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(s_part, r) + 2 * head);
-                            x[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_acc, r) + head * (D + 4) + d);
-                        }
-                    float top = ml[0].x;
-#pragma unroll
-                    for (int r = 1; r < kMaxCluster; ++r)
-                        if (r < p.ctas) top = fmaxf(top, ml[r].x);
-                    const float ref = top == __int_as_float(0xff800000) ? 0.0f : top;
+                    float top = __int_as_float(0xff800000), sum = 0.0f;
                     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float sum = 0.0f;
+                    for (int r0 = 0; r0 < p.ctas; r0 += 8) {          // eight CTAs at a time
+                        float2 ml[8];
+                        float4 x[8];
 #pragma unroll
-                    for (int r = 0; r < kMaxCluster; ++r)
-                        if (r < p.ctas) {
-                            const float a = exp2_approx(ml[r].x - ref);
-                            sum += a * ml[r].y;
-                            o.x += a * x[r].x;
-                            o.y += a * x[r].y;
-                            o.z += a * x[r].z;
-                            o.w += a * x[r].w;
-                        }
+                        for (int r = 0; r < 8; ++r)
+                            if (r0 + r < p.ctas) {
+                                ml[r] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(s_part, r0 + r) + 2 * head);
+                                x[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_acc, r0 + r) +
+                                                                        head * (D + 4) + d);
+                            }
+                        float to = top;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+                            if (r0 + r < p.ctas) to = fmaxf(to, ml[r].x);
+                        const float ref = to == __int_as_float(0xff800000) ? 0.0f : to;
+                        const float down = exp2_approx(top - ref);
+                        top = to;
+                        sum *= down;
+                        o.x *= down;
+                        o.y *= down;
+                        o.z *= down;
+                        o.w *= down;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+                            if (r0 + r < p.ctas) {
+                                const float a = exp2_approx(ml[r].x - ref);
+                                sum += a * ml[r].y;
+                                o.x += a * x[r].x;
+                                o.y += a * x[r].y;
+                                o.z += a * x[r].z;
+                                o.w += a * x[r].w;
+                            }
+                    }
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                     QT* dst = out + (static_cast<size_t>(was.b) * heads_total + was_head0 + head) * D + d;
                     *reinterpret_cast<uint2*>(dst) =
@@ -915,6 +924,9 @@ cudaError_t launch(const AttendParams& p, AttendForm form, cudaStream_t st) {
     if (form == kAttendCluster) {
         static SmemLimit limit;
         cudaError_t e = limit.ensure(attend_kernel<QBF, I8, D, NT, true>, S::kShared);
+        if (e == cudaSuccess && p.ctas > 8)
+            e = cudaFuncSetAttribute(attend_kernel<QBF, I8, D, NT, true>,
+                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(p.B * p.H * p.chunks * p.ctas);

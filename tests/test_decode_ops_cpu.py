@@ -60,7 +60,7 @@ def test_paged_append_refusals():
     refused(append(k=ctypes.c_void_p(0x1008)), "16-byte")
 
 
-def attend(q=P, stride=128, kind=0, cache=0, B=1, H=1, group=2, D=64, W=256, page=16, n_pages=8,
+def attend(q=P, stride=128, kind=0, cache=0, B=1, H=1, group=2, D=64, W=1024, page=16, n_pages=8,
            work=P, nbytes=1 << 30):
     return lib.escha_paged_attend(q, stride, 64, kind, P, P, cache, None, None, P, P, B, H, group, D, W,
                                   page, n_pages, 1.0, work, nbytes, P, None)
@@ -85,11 +85,12 @@ def test_workspace_is_asked_for_only_when_a_second_launch_joins():
     size = lib.escha_paged_attend_workspace_bytes
     assert size(1000, 2, 8, 256, 4, 16) == 0         # 64 tokens: one block, never cut
     assert size(8, 2, 8, 256, 128, 16) == 0          # short rows, few enough: clusters
-    # 3200 tokens are 50 blocks: a CTA for each of both heads' (two fit each of 148 SMs), two
-    # pieces of 8 heads per CTA, each with its maximum, sum and channels
-    ctas = 100
-    assert size(1, 2, 8, 256, 200, 16) == ctas * 8 + 2 * ctas * 8 * (8 + 4 * 256)
-    assert size(0, 2, 8, 256, 200, 16) == size(1, 2, 8, 256, 200, 20) == 0
+    assert size(4, 2, 8, 256, 512, 16) == 0          # 8192 tokens: a few rows, wide clusters
+    # 9600 tokens are 150 blocks of both heads: two CTAs for each of 148 SMs, two pieces of 8
+    # heads per CTA, each with its maximum, sum and channels
+    ctas = 296
+    assert size(1, 2, 8, 256, 600, 16) == ctas * 8 + 2 * ctas * 8 * (8 + 4 * 256)
+    assert size(0, 2, 8, 256, 600, 16) == size(1, 2, 8, 256, 600, 20) == 0
 
 
 def test_python_level_refusals_without_a_gpu():

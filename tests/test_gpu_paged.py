@@ -348,11 +348,12 @@ def test_attend_short_rows_of_wide_tables(cuda, lens):
 
 
 @pytest.mark.parametrize("cache,kind", TYPES)
-@pytest.mark.parametrize("b,h", [(400, 1), (37, 2), (100, 1), (20, 8), (3, 99)])
+@pytest.mark.parametrize("b,h", [(400, 1), (37, 2), (100, 1), (20, 8), (3, 99), (4, 2), (1, 8)])
 def test_attend_every_way_of_sharing_rows(cuda, cache, kind, b, h):
     rng = np.random.default_rng(b)
     Case(cuda, rng.integers(0, 65, b), h, 2, 64, 16, cache, kind, spare=0).check()     # one block
     Case(cuda, rng.integers(0, 600, b), h, 2, 64, 16, cache, kind, spare=0).check()
+    Case(cuda, rng.integers(0, 600, b), h, 2, 64, 16, cache, kind, spare=100).check()
 
 
 def test_attend_requests_that_share_pages(cuda):
