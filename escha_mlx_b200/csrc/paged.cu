@@ -183,8 +183,8 @@ __device__ __forceinline__ uint32_t code_of(float x, float scale, float guess, f
 
 constexpr int kAppendThreads = 256;
 // Items of a thread in flight: slots, then rows, then stores.  One at a time: 25.0 us for 131 MB
-// (16001 rows of 8 heads of 128, scattered slots), four 23.9 (5.5 TB/s).
-constexpr int kAppendBatch = 4;
+// (16001 rows of 8 heads of 128, scattered slots), two 22.9 (5.7 TB/s), four 23.9.
+constexpr int kAppendBatch = 2;
 
 // T: type of the rows; Q: 8-bit cache.  Item = 8 elements of one row of one head of k or v;
 // fewer than 2^31 of them.
