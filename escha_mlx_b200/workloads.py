@@ -9,6 +9,8 @@ stream decodes with exactly the same instruction and byte counts as a trained on
   decode step (16 query heads, 2 key/value heads, head size 256).
 * ``moe_stack`` -- several such layers with distinct weights, so that a pass over
   the stack never finds a layer's bytes in L2.
+* ``DecodeStack`` -- the stack's decode step end to end, with paged attention,
+  vocabulary head and sampling.
 """
 from __future__ import annotations
 
@@ -140,3 +142,52 @@ def moe_stack(n_layers: int, device, seed: int = 1234, attention: bool = False,
     gen_experts.manual_seed(seed + 1 + rank)
     return [MoeLayer(device, gen, cfg, attention, expert_range, gen_experts, peer_group)
             for _ in range(n_layers)]
+
+
+class DecodeStack:
+    """The decode step of a layer stack end to end, one new token per request and call: page plan,
+    int8 embedding, the layers with attention over their paged caches (``MoeLayer.decode``) and a
+    residual and RMS norm after each as in the benchmark's step, vocabulary head, sampling.
+
+    Everything a step changes (page table, lengths, position in the free list, tokens, caches) is
+    device state of this object, updated in place and in stream order, so a step can be captured
+    in a CUDA graph and replayed.  Requests that find no free page are refused by the plan and
+    keep their length; ``refused`` holds their number after a step.
+    """
+
+    def __init__(self, layers: list[MoeLayer], embed: quant.EschaQ8Embedding, head: quant.EschaQ8Head,
+                 batch: int, n_pages: int, page_size: int, max_tokens: int,
+                 cache_dtype=torch.float16) -> None:
+        self.layers, self.embed, self.head = layers, embed, head
+        dev = head._w8.device
+        self.page_size, self.n_pages = page_size, n_pages
+        self.caches = [layer.new_cache(n_pages, page_size, cache_dtype) for layer in layers]
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.table = torch.full((batch, -(-max_tokens // page_size)), -1, **i32)
+        self.free_pages = torch.arange(n_pages, **i32)
+        self.taken = torch.zeros(1, **i32)
+        self.lengths = torch.zeros(batch, **i32)
+        self.refused = torch.zeros(1, **i32)
+        self.tokens = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self._one = torch.ones(batch, **i32)
+
+    def state(self) -> list[torch.Tensor]:
+        """What a step changes apart from the caches."""
+        return [self.table, self.taken, self.lengths, self.refused, self.tokens]
+
+    def step(self, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+        """One token per request from ``uniforms`` [batch]; the settings as in
+        ``sampling.sample``.  Returns (and keeps) the tokens [batch]."""
+        from . import paged
+        plan = paged.plan_pages(self.table, self.lengths, self._one, self.free_pages, self.taken,
+                                page_size=self.page_size, n_pages=self.n_pages,
+                                rows=self.tokens.shape[0])
+        x = self.embed(self.tokens)
+        for layer, cache in zip(self.layers, self.caches):
+            x = x + layer.decode(x, cache, self.table, plan)
+            x = torch.nn.functional.rms_norm(x, (x.shape[-1],), eps=1e-6)
+        self.tokens.copy_(self.head.sample(x, uniforms, temperature, top_k, top_p, min_p))
+        self.lengths.copy_(plan.ends)
+        self.taken.copy_(plan.head)
+        self.refused.copy_(plan.refused)
+        return self.tokens

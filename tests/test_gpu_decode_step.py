@@ -14,79 +14,73 @@ CFG = dict(hidden=256, inter=128, experts=8, top_k=2, K_gate_up=2, K_down=2, q_h
 VOCAB, B, PAGE, PAGES, STEPS = 1000, 3, 16, 24, 40
 
 
-class Decoder:
-    def __init__(self, device, dtype):
-        self.layers = workloads.moe_stack(2, device, seed=5, attention=True, cfg=CFG)
-        gen = torch.Generator(device=device).manual_seed(11)
-        lin = workloads._q8(VOCAB, CFG["hidden"], device, gen)
-        self.head = quant.EschaQ8Head(lin._w8, lin._scale)
-        self.embed = quant.EschaQ8Embedding(lin._w8, (lin._scale.float() * 16).half())
-        self.caches = [x.new_cache(PAGES, PAGE, dtype) for x in self.layers]
-        i32 = dict(dtype=torch.int32, device=device)
-        self.table = torch.full((B, 6), -1, **i32)
-        self.free = torch.randperm(PAGES, device=device, generator=gen).to(torch.int32)
-        self.lens, self.pos = torch.zeros(B, **i32), torch.zeros(1, **i32)
-        self.one = torch.ones(B, **i32)
-        self.tokens = torch.tensor([1, 2, 3], device=device)
-        self.u = torch.zeros(B, device=device)
-
-    def step(self):
-        plan = paged.plan_pages(self.table, self.lens, self.one, self.free, self.pos, page_size=PAGE,
-                                n_pages=PAGES, rows=B)
-        x = self.embed(self.tokens)
-        for layer, cache in zip(self.layers, self.caches):
-            x = torch.nn.functional.rms_norm(layer.decode(x, cache, self.table, plan),
-                                             (CFG["hidden"],), eps=1e-6)
-        self.tokens.copy_(self.head.sample(x, self.u, 0.9, 50, 0.95))
-        self.lens.copy_(plan.ends)
-        self.pos.copy_(plan.head)
-        return plan
+def stack(device, dtype, pages=PAGES):
+    layers = workloads.moe_stack(2, device, seed=5, attention=True, cfg=CFG)
+    gen = torch.Generator(device=device).manual_seed(11)
+    lin = workloads._q8(VOCAB, CFG["hidden"], device, gen)
+    emb = workloads._q8(VOCAB, CFG["hidden"], device, gen)   # untied: a tied one repeats its token
+    d = workloads.DecodeStack(layers, quant.EschaQ8Embedding(emb._w8, (emb._scale.float() * 16).half()),
+                              quant.EschaQ8Head(lin._w8, lin._scale), B, pages, PAGE, 6 * PAGE, dtype)
+    d.free_pages.copy_(torch.randperm(pages, device=device, generator=gen))
+    d.tokens.copy_(torch.tensor([1, 2, 3], device=device))
+    return d
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.int8])
 def test_replayed_steps_equal_eager_ones(cuda, dtype):
     gen = torch.Generator(device=cuda).manual_seed(3)
     us = torch.rand((STEPS, B), device=cuda, generator=gen)
-    eager, runs = Decoder(cuda, dtype), []
+    settings = (0.9, 50, 0.95)
+    eager, runs = stack(cuda, dtype), []
     for u in us:
-        eager.u.copy_(u)
-        plan = eager.step()
-        assert plan.refused.item() == 0
-        runs.append(eager.tokens.clone())
-    assert eager.lens.tolist() == [STEPS] * B and eager.pos.item() == B * -(-STEPS // PAGE)
+        runs.append(eager.step(u, *settings).clone())
+        assert eager.refused.item() == 0
+    assert eager.lengths.tolist() == [STEPS] * B and eager.taken.item() == B * -(-STEPS // PAGE)
     assert len({tuple(t.tolist()) for t in runs}) > STEPS // 2      # it does not stand still
 
-    graphed = Decoder(cuda, dtype)
-    saved = [t.clone() for t in (graphed.table, graphed.lens, graphed.pos, graphed.tokens)]
+    graphed = stack(cuda, dtype)
+    saved = [t.clone() for t in graphed.state()]
+    u = torch.zeros(B, device=cuda)
     graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
-        graphed.step()                                              # sizes workspaces
+        graphed.step(u, *settings)                                  # sizes workspaces
     stream.synchronize()
     with torch.cuda.graph(graph, stream=stream):
-        graphed.step()
-    for t, s in zip((graphed.table, graphed.lens, graphed.pos, graphed.tokens), saved):
+        graphed.step(u, *settings)
+    for t, s in zip(graphed.state(), saved):
         t.copy_(s)
     for c in graphed.caches:
         for a in c.arrays():
             a.zero_()
-    for u, want in zip(us, runs):
-        graphed.u.copy_(u)
+    for now, want in zip(us, runs):
+        u.copy_(now)
         graph.replay()
         assert torch.equal(graphed.tokens, want)
     for a, b in zip(eager.caches, graphed.caches):
         assert all(torch.equal(x, y) for x, y in zip(a.arrays(), b.arrays()))
 
 
+def test_requests_without_a_page_keep_their_length(cuda):
+    """Five pages for three requests: when all have filled one, only two more are served."""
+    d = stack(cuda, torch.float16, pages=5)
+    u = torch.full((B,), 0.5, device=cuda)
+    for step in range(20):
+        d.step(u, 0.9)
+    # 16 tokens each in the first three pages, then two pages more: requests 0 and 1
+    assert d.lengths.tolist() == [20, 20, 16] and d.refused.item() == 1 and d.taken.item() == 5
+
+
 def test_layer_attends_to_its_history(cuda):
     """The layer's attention against a plain one over the projections of every earlier input."""
-    d = Decoder(cuda, torch.float16)
+    d = stack(cuda, torch.float16)
+    one = torch.ones(B, dtype=torch.int32, device=cuda)
     layer, cache = d.layers[0], d.caches[0]
     gen = torch.Generator(device=cuda).manual_seed(9)
     ks, vs = [], []
     for step in range(20):
         x = torch.randn((B, CFG["hidden"]), device=cuda, generator=gen).half()
-        plan = paged.plan_pages(d.table, d.lens, d.one, d.free, d.pos, page_size=PAGE, n_pages=PAGES,
+        plan = paged.plan_pages(d.table, d.lengths, one, d.free_pages, d.taken, page_size=PAGE, n_pages=PAGES,
                                 rows=B)
         got = layer.attend(x, cache, d.table, plan)
         q, k, v = (lin(x).double().view(B, -1, 64) for lin in (layer.q, layer.k, layer.v))
@@ -104,4 +98,4 @@ def test_layer_attends_to_its_history(cuda):
         assert bool(((got.double().view_as(want) - want).abs() <= tol).all())
         out = layer.decode(x, cache, d.table, plan)      # stores the same rows again
         assert torch.equal(out, layer.block(torch.add(x, layer.o(got), alpha=0.01)))
-        d.lens, d.pos = plan.ends, plan.head
+        d.lengths, d.taken = plan.ends, plan.head
