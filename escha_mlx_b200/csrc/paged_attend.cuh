@@ -236,8 +236,14 @@ __global__ void __launch_bounds__(kThreads, Shape<QBF, I8, D, NT>::kResident) at
     long long total = 0, shares = 0, u = 0, u_end = 1;
     if constexpr (!CL) {
         total = static_cast<long long>(s_prefix[p.B]) * per_request;
-        // as many CTAs as there are blocks at most, so that no share is empty
+        // As many CTAs as there are blocks at most, so that no share is empty, and no more than
+        // the largest share asks for: fewer pieces to join (one request of 9000 tokens, 2 heads of
+        // 256: 15.5 us against 19.0; no difference with many blocks per CTA).
         shares = min(static_cast<long long>(p.ctas), total);
+        if (shares > 0) {
+            const long long most = (total + shares - 1) / shares;
+            shares = (total + most - 1) / most;
+        }
         u = c < shares ? total * c / shares : 0;
         u_end = c < shares ? total * (c + 1) / shares : 0;
         // requests without a token: zeros
