@@ -6,17 +6,18 @@
 //   token = first index, in index order, whose cumulative kept weight exceeds u * total.
 //
 // The token is a whole number that has to come out the same whatever the split, so weights are
-// computed in 64 bits and summed as fixed-point integers of 44 fractional bits (262144 of them
-// stay far below 2^64): sums do not depend on their order, borders move by 2^-45 per token.
+// computed in 64 bits and summed as fixed-point integers of 44 fractional bits (the longest row
+// has fewer than 2^20 tokens, so a sum stays below 2^64): sums do not depend on their order,
+// borders move by 2^-45 per token.
 //
 // A thread-block cluster holds one row in the shared memory of its CTAs (the row is read from
 // HBM once) and agrees on maxima, counts and sums through distributed shared memory.  Nothing
 // is sorted as a whole: a histogram over 1023 bins of d (monotone in x) bounds the part of the
 // row that can be kept, from counts alone (a bin's weights differ by 3%, so the nucleus is
-// bounded from above).  Where at most kList tokens are left, one CTA sorts those and settles
-// everything exactly; otherwise the cut is found bin by bin, from exact weights per bin, and
-// inside its bin by sorting it or, if ties make it large, by halving the range of values.
-// Bound by latency at small batches, by the 64-bit exponentials at large ones.
+// bounded from above).  Where at most kList tokens are left, one CTA settles those exactly;
+// otherwise the cut is found bin by bin, from exact weights per bin, and inside its bin by finer
+// buckets or, if ties make it large, by halving the range of values.
+// Bound by the latency of those exchanges (barriers are the top stall; the 64-bit pipe is 7% busy).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -82,7 +83,6 @@ struct Shared {
     uint32_t ties;                          // this CTA's tokens at the cut
     uint32_t count;                         // a count exchanged between CTAs
     uint32_t found, found2;                 // a thread's find, for its CTA
-    uint32_t found_above;
     uint32_t list_n;                        // (leader) tokens in the list
     uint32_t cut_key;                       // (leader) the cut, for all CTAs
     uint32_t cut_ties;

@@ -197,7 +197,9 @@ def test_longest_rows(cuda):
     for kind in ("f16", "f32"):
         v = sampling.max_vocab(DT[kind])
         x, u = logits_of(cuda, 2, v, kind, seed=5)
-        for s in ((0.7, 50, 0.9, 0.0), (2.0, 0, 0.999, 0.0), (1.0, 0, 1.0, 0.0)):
+        # at the last temperatures every token weighs as much as the largest
+        for s in ((0.7, 50, 0.9, 0.0), (2.0, 0, 0.999, 0.0), (1.0, 0, 1.0, 0.0), (1e30, 0, 1.0, 0.0),
+                  (1e30, 0, 0.97, 0.0), (1e30, v - 7, 1.0, 0.0)):
             check(sampling.sample(x, u, *s), x, u, *s)
         with pytest.raises(ValueError, match="V="):
             sampling.sample(torch.zeros((1, v + 1), dtype=DT[kind], device=cuda), u[:1])
